@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(_HERE, "libcleave_cuda.so")
 c_buf = ctypes.c_void_p
 c_f32p = ctypes.POINTER(ctypes.c_float)
 c_f64p = ctypes.POINTER(ctypes.c_double)
+c_u8p = ctypes.POINTER(ctypes.c_uint8)
 f64 = ctypes.c_double
 i32, i64, f32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 
@@ -124,6 +125,16 @@ SIGNATURES = {
     "cleave_cuda_colsum_f64": (c_buf, [c_buf, i32, i32]),
     "cleave_cuda_mse_f64": (f64, [c_buf, c_buf, c_buf]),
     "cleave_cuda_sgd_f64": (i32, [c_buf, c_buf, f64, f64]),
+    "cleave_cuda_e4m3_bytes": (i64, [i32, i32]),
+    "cleave_cuda_e4m3_scales": (i64, [i32, i32, i32]),
+    "cleave_cuda_alloc_e4m3": (c_buf, [i64]),
+    "cleave_cuda_wrap_e4m3": (c_buf, [ctypes.c_void_p, i64]),
+    "cleave_cuda_upload_e4m3": (c_buf, [c_u8p, i64]),
+    "cleave_cuda_download_e4m3": (i64, [c_buf, c_u8p, i64]),
+    "cleave_cuda_quantize_e4m3": (i32, [c_buf, i32, i32, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf]),
+    "cleave_cuda_dequantize_e4m3": (i32, [c_buf, c_buf, c_buf, i32, i32, i32]),
+    "cleave_cuda_gemm_e4m3": (i32, [c_buf, c_buf, c_buf, i32, c_buf, c_buf, i32, i32, i32, i32, i32, i32, c_buf, i32]),
+    "cleave_cuda_act_bwd_e4m3": (i32, [c_buf, c_buf, i32, c_buf, i32, i32, i32, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf]),
     "cleave_cuda_dp_sgd_allreduce_f32": (i32, [ctypes.POINTER(ctypes.c_void_p)] * 3 + [ctypes.c_void_p, ctypes.c_void_p,
                                                 i64, i64, i32, i32, f32, ctypes.c_uint32, ctypes.c_void_p]),
     "cleave_cuda_linreg_step_f32": (f32, [c_buf, c_buf, c_buf, c_buf, c_buf, i32, i32]),

@@ -23,7 +23,7 @@ def rust_type(t) -> str:
     if t is None:
         return "()"
     table = {ctypes.c_int32: "i32", ctypes.c_int64: "i64", ctypes.c_float: "f32", ctypes.c_double: "f64",
-             ctypes.c_uint32: "u32", ctypes.c_uint64: "u64",
+             ctypes.c_uint32: "u32", ctypes.c_uint64: "u64", ctypes.c_uint8: "u8",
              ctypes.c_void_p: "*mut c_void", ctypes.c_char_p: "*const c_char"}
     if t in table:
         return table[t]

@@ -10,7 +10,8 @@
 
 namespace cleave {
 
-enum { DT_F32 = 0, DT_F64 = 1 };
+enum { DT_F32 = 0, DT_F64 = 1, DT_E4M3 = 2 };   // E4M3: bytes of a block-scaled 8-bit tensor (quant.cuh)
+inline int64_t dtype_bytes(int dtype) { return dtype == DT_F64 ? 8 : dtype == DT_E4M3 ? 1 : 4; }
 
 // One device tensor: dense row-major, `len` elements of `dtype` at `ptr` (f64 entry points cast).
 struct Buf {
@@ -24,7 +25,7 @@ struct Buf {
   cudaEvent_t xfer_ev;
   cudaEvent_t order_ev;
   bool xfer_pending;
-  int dtype;          // DT_F32 or DT_F64
+  int dtype;          // DT_F32, DT_F64 or DT_E4M3
 };
 constexpr uint32_t kMagic = 0xC1EA7E5Bu;
 
@@ -68,6 +69,7 @@ struct ApiLock {
 
 // ---- handles and memory ---------------------------------------------------------------
 Buf* new_buf(int64_t len, int dtype = DT_F32);   // pooled device allocation; nullptr + error on failure
+Buf* new_view(void* device_ptr, int64_t len, int dtype);   // non-owning handle over caller memory
 // Validates the handle and its element type, settles a pending async transfer; nullptr + error on failure.
 Buf* as_buf(cleave_buf h, const char* what, int dtype = DT_F32);
 Buf* lookup_buf(cleave_buf h, const char* what);   // validates liveness only

@@ -560,11 +560,12 @@ bool split_lo_plane(const float* src, float* dst, int64_t n, cudaStream_t on_str
   return cuda_ok(cudaGetLastError(), "lo-plane split launch");
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_tiled_fn() {
+EncodeTiledFn encode_tiled_fn() {
+  // The encoder is a driver call and needs a current context; a host thread whose first CUDA call this is has none yet.
+  if (cudaSetDevice(ctx().device) != cudaSuccess) {
+    cudaGetLastError();
+    return nullptr;
+  }
   static EncodeTiledFn fn = nullptr;
   if (!fn) {
     void* p = nullptr;

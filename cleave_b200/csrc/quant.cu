@@ -1,0 +1,504 @@
+// Block quantization to 8 bits, its inverse, and the derivative form of an activation that was kept in 8 bits.
+//
+// One kernel does all the writing.  A CTA takes a 128 x 128 tile, one block of every form, holds it in registers (64 values a
+// thread, loaded as 16 independent 16-byte words) and makes each form that is asked for from that one read: a warp owns 16
+// whole rows of the tile, so a 1 x 128 block's maximum is one warp reduction, and a 128 x 1 block's is a maximum over the
+// warp's 16 rows in a register and over the 8 warps in shared memory.  HBM bound: 4 bytes read (5 with a checkpoint) and one
+// byte written per element and form.
+//
+// Scale of a block: s = 2^e with e = ceil(log2(amax / 448)), the smallest power of two that brings the block's largest
+// magnitude to at most 448 = 1.75 * 2^8.  With amax = m * 2^E (1 <= m < 2) that is e = E - 8, or E - 7 where m > 1.75: an
+// integer addition that carries into the exponent field exactly when the mantissa is above 1.75's.  A power of two costs
+// no precision (e4m3 is a floating-point format: only values 2^14 below the block's maximum reach its subnormals) and makes
+// x / s, q * s and a later sum of products scaled by s exact.  e is clamped to [-126, 120]; amax = 0 gives -126.
+//
+// Non-finite values: they do not count for the maximum and are stored as NaN, so one infinity shows up as one NaN, and in
+// the sums it takes part in, instead of flushing its block to zero or passing as 448.
+#include <cmath>
+
+#include "common.cuh"
+#include "quant.cuh"
+
+namespace cleave {
+
+constexpr int kQThreads = 256;
+constexpr int kQWarps = kQThreads / 32;
+constexpr int kQRows = kQBlock / kQWarps;   // rows of the tile per warp
+
+struct TileArgs {
+  int rows, cols;
+  int vec;                // x (and dz) are 16-byte aligned and cols is a multiple of 4
+  const float* x;         // [rows, cols]: the values, or the upstream gradient
+  const uint8_t* y_q;     // checkpoint of the activation's output (null: plain quantization)
+  const float* y_s;
+  int y_blocks, act;
+  float* dz;              // outputs, each may be null
+  uint8_t *q_rows, *q_cols, *q_tiles;
+  float *s_rows, *s_cols, *s_tiles;
+  float* db_part;         // [row blocks][cols]: column sums of each row block
+};
+
+// |v| as an ordered integer; 0 for a non-finite v.
+__device__ __forceinline__ uint32_t finite_abs_bits(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+
+// Biased exponent of the block's scale, in [1, 247].
+__device__ __forceinline__ uint32_t scale_exponent(uint32_t amax_bits) {
+  const int e = (int)((amax_bits + 0x1fffffu) >> 23) - 8;   // E - 8 (biased), + 1 where the mantissa is above 1.75's
+  return (uint32_t)(e < 1 ? 1 : e);
+}
+__device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float(e << 23); }
+__device__ __forceinline__ float inverse_scale_of(uint32_t e) { return __uint_as_float((254u - e) << 23); }
+
+// Two values to two e4m3 bytes (lo in the low byte), round to nearest even.
+__device__ __forceinline__ uint32_t e4m3x2(float hi, float lo) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float scaled(float v, float inv) {
+  return finite_abs_bits(v) == 0u && v != 0.0f ? __uint_as_float(0x7fc00000u) : __fmul_rn(v, inv);
+}
+__device__ __forceinline__ uint32_t quantize4(const float (&v)[4], const float (&inv)[4]) {
+  return e4m3x2(scaled(v[1], inv[1]), scaled(v[0], inv[0])) | (e4m3x2(scaled(v[3], inv[3]), scaled(v[2], inv[2])) << 16);
+}
+// Four e4m3 bytes to f32 (exact).
+__device__ __forceinline__ void unpack4(uint32_t w, float (&v)[4]) {
+  uint32_t a, b;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(a) : "h"((uint16_t)(w & 0xffffu)));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"((uint16_t)(w >> 16)));
+  asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; cvt.f32.f16 %0, l; cvt.f32.f16 %1, h;}" : "=f"(v[0]), "=f"(v[1]) : "r"(a));
+  asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; cvt.f32.f16 %0, l; cvt.f32.f16 %1, h;}" : "=f"(v[2]), "=f"(v[3]) : "r"(b));
+}
+
+// act'(y) * g with every step rounded as the f32 derivative forms round it (elementwise.cu).
+__device__ __forceinline__ float act_grad(float y, float g, int act) {
+  switch (act) {
+    case CLEAVE_ACT_TANH: return __fmul_rn(__fsub_rn(1.0f, __fmul_rn(y, y)), g);
+    case CLEAVE_ACT_SIGMOID: return __fmul_rn(__fmul_rn(y, __fsub_rn(1.0f, y)), g);
+    case CLEAVE_ACT_RELU: return y > 0.0f ? g : 0.0f;
+    default: return g;
+  }
+}
+
+template <bool CHECKPOINT>
+__global__ void __launch_bounds__(kQThreads, 2) tile_kernel(const TileArgs a) {
+  __shared__ uint32_t s_max[kQWarps][kQBlock];
+  __shared__ float s_sum[kQWarps][kQBlock];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int col_blocks = (a.cols + kQBlock - 1) / kQBlock;
+  const int rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
+  const int r0 = rb * kQBlock + warp * kQRows, c0 = cb * kQBlock + lane * 4;
+  const int64_t pitch = ((int64_t)a.cols + 15) / 16 * 16;
+
+  float v[kQRows][4];
+#pragma unroll
+  for (int i = 0; i < kQRows; ++i) {
+    const int r = r0 + i;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[i][j] = 0.0f;
+    if (r < a.rows) {
+      const float* src = a.x + (int64_t)r * a.cols + c0;
+      if (a.vec) {
+        if (c0 < a.cols) {
+          const float4 t = __ldcs(reinterpret_cast<const float4*>(src));
+          v[i][0] = t.x; v[i][1] = t.y; v[i][2] = t.z; v[i][3] = t.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c0 + j < a.cols) v[i][j] = __ldg(src + j);
+      }
+    }
+  }
+  if constexpr (CHECKPOINT) {
+    float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (a.y_blocks == CLEAVE_BLOCKS_COLS) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c0 + j < a.cols) sc[j] = __ldg(a.y_s + (int64_t)rb * a.cols + c0 + j);
+    } else if (a.y_blocks == CLEAVE_BLOCKS_TILES) {
+      sc[0] = sc[1] = sc[2] = sc[3] = __ldg(a.y_s + (int64_t)rb * col_blocks + cb);
+    }
+#pragma unroll
+    for (int i = 0; i < kQRows; ++i) {
+      const int r = r0 + i;
+      if (r < a.rows && c0 < a.cols) {
+        const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(a.y_q + r * pitch + c0));
+        if (a.y_blocks == CLEAVE_BLOCKS_ROWS) sc[0] = sc[1] = sc[2] = sc[3] = __ldg(a.y_s + (int64_t)cb * a.rows + r);
+        float y[4];
+        unpack4(w, y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[i][j] = c0 + j < a.cols ? act_grad(__fmul_rn(y[j], sc[j]), v[i][j], a.act) : 0.0f;   // padding bytes may be anything
+      }
+    }
+    if (a.dz != nullptr) {
+#pragma unroll
+      for (int i = 0; i < kQRows; ++i) {
+        const int r = r0 + i;
+        if (r < a.rows) {
+          float* dst = a.dz + (int64_t)r * a.cols + c0;
+          if (a.vec) {
+            if (c0 < a.cols) *reinterpret_cast<float4*>(dst) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (c0 + j < a.cols) dst[j] = v[i][j];
+          }
+        }
+      }
+    }
+  }
+
+  // ---- 1 x 128 blocks: a row of the tile is one warp's
+  if (a.q_rows != nullptr) {
+    float own_scale = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kQRows; ++i) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m = max(m, finite_abs_bits(v[i][j]));
+      const uint32_t e = scale_exponent(__reduce_max_sync(0xffffffffu, m));
+      if (lane == i) own_scale = scale_of(e);
+      const float inv = inverse_scale_of(e);
+      const float inv4[4] = {inv, inv, inv, inv};
+      const int r = r0 + i;
+      if (r < a.rows && c0 < pitch) *reinterpret_cast<uint32_t*>(a.q_rows + r * pitch + c0) = quantize4(v[i], inv4);
+    }
+    if (lane < kQRows && r0 + lane < a.rows) a.s_rows[(int64_t)cb * a.rows + r0 + lane] = own_scale;
+  }
+
+  // ---- what needs the whole tile: column maxima, the tile's maximum, column sums
+  if (a.q_cols == nullptr && a.q_tiles == nullptr && a.db_part == nullptr) return;
+  uint32_t m[4] = {0, 0, 0, 0};
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < kQRows; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = max(m[j], finite_abs_bits(v[i][j]));
+      sum[j] = __fadd_rn(sum[j], v[i][j]);
+    }
+  *reinterpret_cast<uint4*>(&s_max[warp][lane * 4]) = make_uint4(m[0], m[1], m[2], m[3]);
+  *reinterpret_cast<float4*>(&s_sum[warp][lane * 4]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+  __syncthreads();
+  if (a.db_part != nullptr && threadIdx.x < kQBlock) {
+    const int c = cb * kQBlock + (int)threadIdx.x;
+    if (c < a.cols) {
+      float t = s_sum[0][threadIdx.x];
+#pragma unroll
+      for (int w = 1; w < kQWarps; ++w) t = __fadd_rn(t, s_sum[w][threadIdx.x]);
+      a.db_part[(int64_t)rb * a.cols + c] = t;
+    }
+  }
+  if (a.q_cols == nullptr && a.q_tiles == nullptr) return;
+#pragma unroll
+  for (int w = 0; w < kQWarps; ++w) {
+    const uint4 t = *reinterpret_cast<const uint4*>(&s_max[w][lane * 4]);
+    m[0] = max(m[0], t.x); m[1] = max(m[1], t.y); m[2] = max(m[2], t.z); m[3] = max(m[3], t.w);
+  }
+  if (a.q_cols != nullptr) {
+    float inv[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t e = scale_exponent(m[j]);
+      inv[j] = inverse_scale_of(e);
+      if (warp == 0 && c0 + j < a.cols) a.s_cols[(int64_t)rb * a.cols + c0 + j] = scale_of(e);
+    }
+#pragma unroll
+    for (int i = 0; i < kQRows; ++i) {
+      const int r = r0 + i;
+      if (r < a.rows && c0 < pitch) *reinterpret_cast<uint32_t*>(a.q_cols + r * pitch + c0) = quantize4(v[i], inv);
+    }
+  }
+  if (a.q_tiles != nullptr) {
+    const uint32_t e = scale_exponent(__reduce_max_sync(0xffffffffu, max(max(m[0], m[1]), max(m[2], m[3]))));
+    const float inv = inverse_scale_of(e);
+    const float inv4[4] = {inv, inv, inv, inv};
+    if (threadIdx.x == 0) a.s_tiles[(int64_t)rb * col_blocks + cb] = scale_of(e);
+#pragma unroll
+    for (int i = 0; i < kQRows; ++i) {
+      const int r = r0 + i;
+      if (r < a.rows && c0 < pitch) *reinterpret_cast<uint32_t*>(a.q_tiles + r * pitch + c0) = quantize4(v[i], inv4);
+    }
+  }
+}
+
+// out[r, c] = q * scale: one thread per four columns of a row.
+__global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ q, const float* __restrict__ s,
+                                                         float* __restrict__ out, int rows, int cols, int blocks, int vec) {
+  const int64_t pitch = ((int64_t)cols + 15) / 16 * 16;
+  const int col_blocks = (cols + kQBlock - 1) / kQBlock;
+  const int groups = (cols + 3) / 4;
+  const int64_t total = (int64_t)rows * groups;
+  for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < total; t += (int64_t)gridDim.x * blockDim.x) {
+    const int r = (int)(t / groups), c = (int)(t - (int64_t)r * groups) * 4;
+    float v[4];
+    unpack4(__ldg(reinterpret_cast<const uint32_t*>(q + r * pitch + c)), v);
+    float sc[4];
+    if (blocks == CLEAVE_BLOCKS_COLS) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sc[j] = c + j < cols ? __ldg(s + (int64_t)(r / kQBlock) * cols + c + j) : 0.0f;
+    } else {
+      sc[0] = blocks == CLEAVE_BLOCKS_ROWS ? __ldg(s + (int64_t)(c / kQBlock) * rows + r)
+                                           : __ldg(s + (int64_t)(r / kQBlock) * col_blocks + c / kQBlock);
+      sc[1] = sc[2] = sc[3] = sc[0];
+    }
+    float* dst = out + (int64_t)r * cols + c;
+    if (vec) {
+      *reinterpret_cast<float4*>(dst) = make_float4(__fmul_rn(v[0], sc[0]), __fmul_rn(v[1], sc[1]), __fmul_rn(v[2], sc[2]),
+                                                    __fmul_rn(v[3], sc[3]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < cols) dst[j] = __fmul_rn(v[j], sc[j]);
+    }
+  }
+}
+
+bool q_operand(cleave_buf q, cleave_buf s, int rows, int cols, int blocks, const char* what, QOperand* out) {
+  if (rows <= 0 || cols <= 0) {
+    set_error(CLEAVE_CUDA_ERR_ARG, "%s: rows and cols must be positive (got %d, %d)", what, rows, cols);
+    return false;
+  }
+  if (blocks < CLEAVE_BLOCKS_ROWS || blocks > CLEAVE_BLOCKS_TILES) {
+    set_error(CLEAVE_CUDA_ERR_ARG, "%s: unknown block form %d", what, blocks);
+    return false;
+  }
+  Buf* Q = as_buf(q, what, DT_E4M3);
+  if (!Q) return false;
+  Buf* S = as_buf(s, what);
+  if (!S) return false;
+  if (Q->len != q_bytes(rows, cols) || S->len != q_scales(rows, cols, blocks)) {
+    set_error(CLEAVE_CUDA_ERR_SHAPE, "%s: %lld bytes and %lld scales given, a %d x %d tensor has %lld and %lld", what,
+              (long long)Q->len, (long long)S->len, rows, cols, (long long)q_bytes(rows, cols),
+              (long long)q_scales(rows, cols, blocks));
+    return false;
+  }
+  if (!aligned16(Q->ptr)) {
+    set_error(CLEAVE_CUDA_ERR_ARG, "%s: the bytes of an 8-bit tensor must be 16-byte aligned", what);
+    return false;
+  }
+  out->q = (uint8_t*)Q->ptr;
+  out->s = S->ptr;
+  return true;
+}
+
+static bool overlaps(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  return a && b && (const char*)a < (const char*)b + b_bytes && (const char*)b < (const char*)a + a_bytes;
+}
+
+bool ranges_distinct(const MemRange* out, int n_out, const MemRange* in, int n_in, const char* what) {
+  for (int i = 0; i < n_out; ++i) {
+    for (int j = i + 1; j < n_out; ++j)
+      if (overlaps(out[i].p, out[i].bytes, out[j].p, out[j].bytes)) {
+        set_error(CLEAVE_CUDA_ERR_ARG, "%s: two outputs share memory", what);
+        return false;
+      }
+    for (int j = 0; j < n_in; ++j)
+      if (overlaps(out[i].p, out[i].bytes, in[j].p, in[j].bytes)) {
+        set_error(CLEAVE_CUDA_ERR_ARG, "%s: an output shares memory with an input", what);
+        return false;
+      }
+  }
+  return true;
+}
+
+static bool launch_tiles(const TileArgs& a, const char* what) {
+  const int64_t tiles = (((int64_t)a.rows + kQBlock - 1) / kQBlock) * (((int64_t)a.cols + kQBlock - 1) / kQBlock);
+  if (tiles > 0x7fffffffll) {
+    set_error(CLEAVE_CUDA_ERR_UNSUPPORTED, "%s: %d x %d has more than 2^31 - 1 blocks", what, a.rows, a.cols);
+    return false;
+  }
+  if (a.y_q)
+    tile_kernel<true><<<(int)tiles, kQThreads, 0, ctx().stream>>>(a);
+  else
+    tile_kernel<false><<<(int)tiles, kQThreads, 0, ctx().stream>>>(a);
+  count_launch();
+  return cuda_ok(cudaGetLastError(), "quantize kernel launch");
+}
+
+}  // namespace cleave
+
+using namespace cleave;
+
+extern "C" {
+
+int64_t cleave_cuda_e4m3_bytes(int32_t rows, int32_t cols) { return rows > 0 && cols > 0 ? q_bytes(rows, cols) : 0; }
+
+int64_t cleave_cuda_e4m3_scales(int32_t rows, int32_t cols, int32_t blocks) {
+  return rows > 0 && cols > 0 ? q_scales(rows, cols, blocks) : 0;
+}
+
+cleave_buf cleave_cuda_alloc_e4m3(int64_t bytes) {
+  ApiLock lock;
+  return (cleave_buf)new_buf(bytes, DT_E4M3);
+}
+
+cleave_buf cleave_cuda_wrap_e4m3(void* device_ptr, int64_t bytes) {
+  ApiLock lock;
+  if (!device_ptr || bytes <= 0 || !aligned16(device_ptr)) {
+    set_error(CLEAVE_CUDA_ERR_ARG, "wrap_e4m3: need a 16-byte aligned device pointer and a positive length");
+    return nullptr;
+  }
+  return (cleave_buf)new_view(device_ptr, bytes, DT_E4M3);
+}
+
+cleave_buf cleave_cuda_upload_e4m3(const uint8_t* host, int64_t bytes) {
+  ApiLock lock;
+  if (!host) {
+    set_error(CLEAVE_CUDA_ERR_ARG, "upload_e4m3: NULL host pointer");
+    return nullptr;
+  }
+  Buf* b = new_buf(bytes, DT_E4M3);
+  if (!b) return nullptr;
+  if (!cuda_ok(cudaMemcpyAsync(b->ptr, host, (size_t)bytes, cudaMemcpyHostToDevice, ctx().stream), "cudaMemcpyAsync(H2D)") ||
+      !cuda_ok(cudaStreamSynchronize(ctx().stream), "cudaStreamSynchronize")) {
+    release_buf(b);
+    return nullptr;
+  }
+  return (cleave_buf)b;
+}
+
+int64_t cleave_cuda_download_e4m3(cleave_buf t, uint8_t* host, int64_t bytes) {
+  ApiLock lock;
+  Buf* b = as_buf(t, "download_e4m3", DT_E4M3);
+  if (!b) return -cleave_cuda_last_error();
+  if (!host || bytes != b->len)
+    return -set_error(CLEAVE_CUDA_ERR_SHAPE, "download_e4m3: room for %lld bytes, tensor has %lld", (long long)bytes,
+                      (long long)b->len);
+  if (!cuda_ok(cudaMemcpyAsync(host, b->ptr, (size_t)bytes, cudaMemcpyDeviceToHost, ctx().stream), "cudaMemcpyAsync(D2H)") ||
+      !cuda_ok(cudaStreamSynchronize(ctx().stream), "cudaStreamSynchronize") || check_device_status() != CLEAVE_CUDA_OK)
+    return -cleave_cuda_last_error();
+  return bytes;
+}
+
+int32_t cleave_cuda_quantize_e4m3(cleave_buf x, int32_t rows, int32_t cols, cleave_buf q_rows, cleave_buf s_rows,
+                                  cleave_buf q_cols, cleave_buf s_cols, cleave_buf q_tiles, cleave_buf s_tiles) {
+  ApiLock lock;
+  if (!ensure_init()) return -cleave_cuda_last_error();   // also makes the library's device this thread's
+  Buf* X = as_buf(x, "quantize");
+  if (!X) return -cleave_cuda_last_error();
+  if (rows <= 0 || cols <= 0 || X->len != (int64_t)rows * cols)
+    return -set_error(CLEAVE_CUDA_ERR_SHAPE, "quantize: tensor has %lld elements, not %d x %d", (long long)X->len, rows, cols);
+  QOperand o[3];
+  const cleave_buf given[3][2] = {{q_rows, s_rows}, {q_cols, s_cols}, {q_tiles, s_tiles}};
+  MemRange out[6];
+  int n_out = 0;
+  for (int f = 0; f < 3; ++f)
+    if (given[f][0] || given[f][1]) {
+      const int blocks = CLEAVE_BLOCKS_ROWS + f;
+      if (!q_operand(given[f][0], given[f][1], rows, cols, blocks, "quantize", &o[f])) return -cleave_cuda_last_error();
+      out[n_out++] = {o[f].q, q_bytes(rows, cols)};
+      out[n_out++] = {o[f].s, q_scales(rows, cols, blocks) * 4};
+    }
+  if (n_out == 0) return -set_error(CLEAVE_CUDA_ERR_ARG, "quantize: no output given");
+  const MemRange in[1] = {{X->ptr, X->len * 4}};
+  if (!ranges_distinct(out, n_out, in, 1, "quantize")) return -cleave_cuda_last_error();
+  Trace tr("quantize", "rows=%d cols=%d", rows, cols);
+  TileArgs a{};
+  a.rows = rows;
+  a.cols = cols;
+  a.vec = aligned16(X->ptr) && cols % 4 == 0;
+  a.x = X->ptr;
+  a.q_rows = o[0].q; a.s_rows = o[0].s;
+  a.q_cols = o[1].q; a.s_cols = o[1].s;
+  a.q_tiles = o[2].q; a.s_tiles = o[2].s;
+  return launch_tiles(a, "quantize") ? CLEAVE_CUDA_OK : -cleave_cuda_last_error();
+}
+
+int32_t cleave_cuda_dequantize_e4m3(cleave_buf out, cleave_buf q, cleave_buf s, int32_t rows, int32_t cols, int32_t blocks) {
+  ApiLock lock;
+  if (!ensure_init()) return -cleave_cuda_last_error();   // also makes the library's device this thread's
+  Buf* O = as_buf(out, "dequantize");
+  if (!O) return -cleave_cuda_last_error();
+  QOperand in;
+  if (!q_operand(q, s, rows, cols, blocks, "dequantize", &in)) return -cleave_cuda_last_error();
+  if (O->len != (int64_t)rows * cols)
+    return -set_error(CLEAVE_CUDA_ERR_SHAPE, "dequantize: output has %lld elements, not %d x %d", (long long)O->len, rows, cols);
+  const MemRange outs[1] = {{O->ptr, O->len * 4}};
+  const MemRange ins[2] = {{in.q, q_bytes(rows, cols)}, {in.s, q_scales(rows, cols, blocks) * 4}};
+  if (!ranges_distinct(outs, 1, ins, 2, "dequantize")) return -cleave_cuda_last_error();
+  Trace tr("dequantize", "rows=%d cols=%d blocks=%d", rows, cols, blocks);
+  dequantize_kernel<<<stream_grid((int64_t)rows * ((cols + 3) / 4), 256, 8), 256, 0, ctx().stream>>>(
+      in.q, in.s, O->ptr, rows, cols, blocks, aligned16(O->ptr) && cols % 4 == 0);
+  count_launch();
+  return cuda_ok(cudaGetLastError(), "dequantize kernel launch") ? CLEAVE_CUDA_OK : -cleave_cuda_last_error();
+}
+
+int32_t cleave_cuda_act_bwd_e4m3(cleave_buf y, cleave_buf y_scale, int32_t y_blocks, cleave_buf g, int32_t rows, int32_t cols,
+                                 int32_t act, cleave_buf dz, cleave_buf q_rows, cleave_buf s_rows, cleave_buf q_cols,
+                                 cleave_buf s_cols, cleave_buf db) {
+  ApiLock lock;
+  if (!ensure_init()) return -cleave_cuda_last_error();   // also makes the library's device this thread's
+  QOperand Y;
+  if (!q_operand(y, y_scale, rows, cols, y_blocks, "act_bwd", &Y)) return -cleave_cuda_last_error();
+  Buf* G = as_buf(g, "act_bwd");
+  if (!G) return -cleave_cuda_last_error();
+  const int64_t n = (int64_t)rows * cols;
+  if (G->len != n)
+    return -set_error(CLEAVE_CUDA_ERR_SHAPE, "act_bwd: gradient has %lld elements, not %d x %d", (long long)G->len, rows, cols);
+  if (act < CLEAVE_ACT_IDENTITY || act > CLEAVE_ACT_TANH)
+    return -set_error(CLEAVE_CUDA_ERR_ARG, "act_bwd: unknown activation code %d", act);
+  MemRange out[6];
+  int n_out = 0;
+  Buf *DZ = nullptr, *DB = nullptr;
+  if (dz) {
+    DZ = as_buf(dz, "act_bwd");
+    if (!DZ) return -cleave_cuda_last_error();
+    if (DZ->len != n)
+      return -set_error(CLEAVE_CUDA_ERR_SHAPE, "act_bwd: dz has %lld elements, not %d x %d", (long long)DZ->len, rows, cols);
+    out[n_out++] = {DZ->ptr, n * 4};
+  }
+  if (db) {
+    DB = as_buf(db, "act_bwd");
+    if (!DB) return -cleave_cuda_last_error();
+    if (DB->len != cols)
+      return -set_error(CLEAVE_CUDA_ERR_SHAPE, "act_bwd: db has %lld elements for %d columns", (long long)DB->len, cols);
+    out[n_out++] = {DB->ptr, (int64_t)cols * 4};
+  }
+  QOperand o[2];
+  const cleave_buf given[2][2] = {{q_rows, s_rows}, {q_cols, s_cols}};
+  for (int f = 0; f < 2; ++f)
+    if (given[f][0] || given[f][1]) {
+      const int blocks = CLEAVE_BLOCKS_ROWS + f;
+      if (!q_operand(given[f][0], given[f][1], rows, cols, blocks, "act_bwd", &o[f])) return -cleave_cuda_last_error();
+      out[n_out++] = {o[f].q, q_bytes(rows, cols)};
+      out[n_out++] = {o[f].s, q_scales(rows, cols, blocks) * 4};
+    }
+  if (n_out == 0) return -set_error(CLEAVE_CUDA_ERR_ARG, "act_bwd: no output given");
+  const MemRange in[3] = {{G->ptr, n * 4}, {Y.q, q_bytes(rows, cols)}, {Y.s, q_scales(rows, cols, y_blocks) * 4}};
+  if (!ranges_distinct(out, n_out, in, 3, "act_bwd")) return -cleave_cuda_last_error();
+  Trace tr("act_bwd_e4m3", "rows=%d cols=%d act=%d", rows, cols, act);
+  TileArgs a{};
+  a.rows = rows;
+  a.cols = cols;
+  a.vec = aligned16(G->ptr) && (!DZ || aligned16(DZ->ptr)) && cols % 4 == 0;
+  a.x = G->ptr;
+  a.y_q = Y.q;
+  a.y_s = Y.s;
+  a.y_blocks = y_blocks;
+  a.act = act;
+  a.dz = DZ ? DZ->ptr : nullptr;
+  a.q_rows = o[0].q; a.s_rows = o[0].s;
+  a.q_cols = o[1].q; a.s_cols = o[1].s;
+  // Column sums: every tile leaves the sums of its 128 rows, a second pass adds the row blocks in ascending order.
+  const int row_blocks = ceil_div(rows, kQBlock);
+  float* part = nullptr;
+  if (DB) {
+    part = row_blocks == 1 ? DB->ptr : scratch_alloc((int64_t)row_blocks * cols * (int64_t)sizeof(float));
+    if (!part) return -cleave_cuda_last_error();
+    a.db_part = part;
+  }
+  bool ok = launch_tiles(a, "act_bwd");
+  if (DB && row_blocks > 1) {
+    ok = ok && colsum_launch(part, DB->ptr, row_blocks, cols, ctx().stream);
+    scratch_free(part);
+  }
+  return ok ? CLEAVE_CUDA_OK : -cleave_cuda_last_error();
+}
+
+}  // extern "C"

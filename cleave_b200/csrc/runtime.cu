@@ -267,6 +267,8 @@ static void pool_free(void* p, int64_t block_bytes) {
   if (!g_capturing) g_cached_bytes += block_bytes;
 }
 
+static const char* dtype_name(int dtype) { return dtype == DT_F64 ? "f64" : dtype == DT_E4M3 ? "e4m3" : "f32"; }
+
 Buf* new_buf(int64_t len, int dtype) {
   if (len <= 0) {
     set_error(CLEAVE_CUDA_ERR_ARG, "tensor length must be positive, got %lld", (long long)len);
@@ -274,11 +276,18 @@ Buf* new_buf(int64_t len, int dtype) {
   }
   if (!ensure_init()) return nullptr;
   int64_t bs = 0;
-  void* p = pool_alloc(len * (int64_t)(dtype == DT_F64 ? sizeof(double) : sizeof(float)), &bs);
+  void* p = pool_alloc(len * dtype_bytes(dtype), &bs);
   if (!p) return nullptr;
   Buf* b = new Buf{kMagic, (float*)p, len, bs, nullptr, nullptr, false, dtype};
   g_live.insert(b);
   g_live_bytes += bs;
+  return b;
+}
+
+Buf* new_view(void* device_ptr, int64_t len, int dtype) {
+  if (!ensure_init()) return nullptr;
+  Buf* b = new Buf{kMagic, (float*)device_ptr, len, 0, nullptr, nullptr, false, dtype};
+  g_live.insert(b);
   return b;
 }
 
@@ -303,7 +312,7 @@ Buf* as_buf(cleave_buf h, const char* what, int dtype) {
   if (!b) return nullptr;
   if (b->dtype != dtype) {
     set_error(CLEAVE_CUDA_ERR_ARG, "%s: tensor holds %s elements, this entry point works on %s", what,
-              b->dtype == DT_F64 ? "f64" : "f32", dtype == DT_F64 ? "f64" : "f32");
+              dtype_name(b->dtype), dtype_name(dtype));
     return nullptr;
   }
   settle_transfer(b);
@@ -721,6 +730,8 @@ int32_t cleave_cuda_upload_async_f32(cleave_buf t, const float* pinned_host, int
   ApiLock lock;
   Buf* b = lookup_buf(t, "upload_async");
   if (!b) return -t_err_code;
+  if (b->dtype == DT_E4M3)   // one byte per element: an f32 copy of its length would overrun it
+    return -set_error(CLEAVE_CUDA_ERR_ARG, "upload_async: tensor holds e4m3 elements, this entry point works on f32");
   if (!pinned_host || len != b->len)
     return -set_error(CLEAVE_CUDA_ERR_SHAPE, "upload_async: %lld elements given, tensor has %lld", (long long)len,
                       (long long)b->len);
@@ -732,6 +743,8 @@ int32_t cleave_cuda_download_async_f32(cleave_buf t, float* pinned_host, int64_t
   ApiLock lock;
   Buf* b = lookup_buf(t, "download_async");
   if (!b) return -t_err_code;
+  if (b->dtype == DT_E4M3)   // one byte per element: an f32 copy of its length would overrun it
+    return -set_error(CLEAVE_CUDA_ERR_ARG, "download_async: tensor holds e4m3 elements, this entry point works on f32");
   if (!pinned_host || len != b->len)
     return -set_error(CLEAVE_CUDA_ERR_SHAPE, "download_async: room for %lld elements, tensor has %lld", (long long)len,
                       (long long)b->len);
@@ -776,10 +789,7 @@ cleave_buf cleave_cuda_wrap_f32(void* device_ptr, int64_t len) {
     set_error(CLEAVE_CUDA_ERR_ARG, "wrap: need a 4-byte aligned device pointer and a positive length");
     return nullptr;
   }
-  if (!ensure_init()) return nullptr;
-  Buf* b = new Buf{kMagic, (float*)device_ptr, len, 0, nullptr, nullptr, false, DT_F32};
-  g_live.insert(b);
-  return (cleave_buf)b;
+  return (cleave_buf)new_view(device_ptr, len, DT_F32);
 }
 
 void* cleave_cuda_data_ptr(cleave_buf t) {

@@ -18,7 +18,7 @@ import math
 
 import numpy as np
 
-from ._lib import c_f32p, c_f64p, lib, raise_last_error
+from ._lib import c_f32p, c_f64p, c_u8p, lib, raise_last_error
 
 _NP = {"f32": np.float32, "f64": np.float64}
 _PTR = {"f32": c_f32p, "f64": c_f64p}
@@ -251,3 +251,171 @@ def gemm_into(c: Tensor, a: Tensor, b: Tensor, *, trans_a=False, trans_b=False, 
     if r != 0:
         raise_last_error("gemm_into")
     return c
+
+
+# ---- 8-bit tensors with a scale per block of 128 ------------------------------------------------------------------
+BLOCKS = {"rows": 1, "cols": 2, "tiles": 3}
+
+
+class QTensor:
+    """A matrix [rows, cols] in 8 bits: e4m3 bytes and one f32 scale per block of 128 (``cleave_cuda_quantize_e4m3``).
+
+    ``blocks`` says which elements share a scale: ``"rows"`` 1 x 128 (an operand whose contraction runs along its rows),
+    ``"cols"`` 128 x 1 (... down its columns), ``"tiles"`` 128 x 128 (weights: either way).  ``scales`` is an f32
+    ``Tensor`` [ceil(cols/128), rows], [ceil(rows/128), cols] or [ceil(rows/128), ceil(cols/128)].  The bytes are
+    row-major with a row pitch of ``cols`` rounded up to 16.
+    """
+
+    __slots__ = ("_h", "scales", "dims", "blocks")
+
+    def __init__(self, rows: int, cols: int, blocks: str, *, _handle=None, _scales: Tensor | None = None):
+        """An uninitialised 8-bit tensor, the destination of ``quantize_into`` / ``nn.act_bwd_q``."""
+        self._h = None
+        self.dims, self.blocks = _q_dims(rows, cols, blocks), blocks
+        if _handle is None:
+            _handle = lib().cleave_cuda_alloc_e4m3(self.nbytes)
+            if not _handle:
+                raise_last_error("QTensor")
+        self._h = _handle
+        self.scales = _scales if _scales is not None else Tensor.empty(*self.scale_dims)
+
+    @classmethod
+    def from_device_ptr(cls, ptr: int, scales_ptr: int, rows: int, cols: int, blocks: str) -> "QTensor":
+        """Non-owning view of caller-owned device memory: the bytes (16-byte aligned, pitch as above) and the scales."""
+        dims = _q_dims(rows, cols, blocks)
+        h = lib().cleave_cuda_wrap_e4m3(ctypes.c_void_p(ptr), lib().cleave_cuda_e4m3_bytes(*dims))
+        if not h:
+            raise_last_error("QTensor")
+        try:
+            scales = Tensor.from_device_ptr(scales_ptr, *_scale_dims(dims, blocks))
+        except Exception:
+            lib().cleave_cuda_free(h)
+            raise
+        return cls(rows, cols, blocks, _handle=h, _scales=scales)
+
+    @classmethod
+    def from_numpy(cls, data: np.ndarray, scales: np.ndarray, cols: int, blocks: str) -> "QTensor":
+        """Uploads e4m3 bytes [rows, pitch] (uint8) and their scales."""
+        data = np.ascontiguousarray(data, np.uint8)
+        if data.ndim != 2:
+            raise TypeError("QTensor: the bytes are a [rows, pitch] array")
+        dims = _q_dims(data.shape[0], cols, blocks)
+        if data.size != lib().cleave_cuda_e4m3_bytes(*dims) or tuple(np.shape(scales)) != _scale_dims(dims, blocks):
+            raise TypeError(f"QTensor: bytes {data.shape} and scales {np.shape(scales)} are not those of {dims}, {blocks!r}")
+        s = Tensor(scales)
+        h = lib().cleave_cuda_upload_e4m3(data.ctypes.data_as(c_u8p), data.size)
+        if not h:
+            raise_last_error("QTensor upload")
+        return cls(*dims, blocks, _handle=h, _scales=s)
+
+    @property
+    def nbytes(self) -> int:
+        """Length of the byte array, padding included."""
+        return int(lib().cleave_cuda_e4m3_bytes(*self.dims))
+
+    @property
+    def scale_dims(self) -> tuple:
+        return _scale_dims(self.dims, self.blocks)
+
+    def numpy(self) -> np.ndarray:
+        """The bytes, [rows, pitch] uint8."""
+        out = np.empty((self.dims[0], self.nbytes // self.dims[0]), np.uint8)
+        if lib().cleave_cuda_download_e4m3(self._h, out.ctypes.data_as(c_u8p), out.size) < 0:
+            raise_last_error("download")
+        return out
+
+    def __del__(self):
+        h, self._h = getattr(self, "_h", None), None
+        if h:
+            try:
+                lib().cleave_cuda_free(h)
+            except Exception:  # interpreter shutdown
+                pass
+
+    def __repr__(self):
+        return f"QTensor<e4m3, {self.dims[0]}, {self.dims[1]}, {self.blocks}>"
+
+
+def _q_dims(rows, cols, blocks) -> tuple:
+    if blocks not in BLOCKS:
+        raise TypeError(f"blocks must be 'rows', 'cols' or 'tiles', not {blocks!r}")
+    if not (1 <= int(rows) < 1 << 31 and 1 <= int(cols) < 1 << 31):   # dims cross the C ABI as i32
+        raise TypeError(f"an 8-bit tensor needs between 1 and 2^31 - 1 rows and columns, not {rows} x {cols}")
+    return int(rows), int(cols)
+
+
+def _scale_dims(dims, blocks) -> tuple:
+    rows, cols = dims
+    rb, cb = -(-rows // 128), -(-cols // 128)
+    return {"rows": (cb, rows), "cols": (rb, cols), "tiles": (rb, cb)}[blocks]
+
+
+def _q_outputs(what: str, dims, outs, forms) -> dict:
+    """``outs`` by block form; each at most once, each of shape ``dims``."""
+    got = {}
+    for o in outs:
+        if not isinstance(o, QTensor) or o.blocks not in forms or o.blocks in got or o.dims != tuple(dims):
+            raise TypeError(f"{what}: cannot write {o!r}: want distinct forms out of {forms} of shape {tuple(dims)}")
+        got[o.blocks] = o
+    return got
+
+
+def _q_handles(got: dict, form: str) -> tuple:
+    o = got.get(form)
+    return (o._h, o.scales._h) if o is not None else (None, None)
+
+
+def quantize_into(x: Tensor, *outs: QTensor) -> None:
+    """Quantizes ``x`` [rows, cols] into each of ``outs`` (one per block form) from one read of it."""
+    if len(x.dims) != 2 or x.dtype != "f32" or not outs:
+        raise TypeError(f"quantize: needs an f32 matrix and at least one output, got {x!r} and {len(outs)}")
+    got = _q_outputs("quantize", x.dims, outs, ("rows", "cols", "tiles"))
+    if lib().cleave_cuda_quantize_e4m3(x._h, *x.dims, *_q_handles(got, "rows"), *_q_handles(got, "cols"),
+                                       *_q_handles(got, "tiles")) != 0:
+        raise_last_error("quantize")
+
+
+def quantize(x: Tensor, *blocks: str):
+    """``x`` in 8 bits, one ``QTensor`` per block form asked for (a tuple when there are several); ``"rows"`` by default."""
+    if len(x.dims) != 2:
+        raise TypeError(f"quantize: needs a matrix, got {x!r}")
+    outs = tuple(QTensor(*x.dims, b) for b in (blocks or ("rows",)))
+    quantize_into(x, *outs)
+    return outs if len(outs) > 1 else outs[0]
+
+
+def dequantize(q: QTensor, out: Tensor | None = None) -> Tensor:
+    """The values ``byte * scale`` as an f32 tensor."""
+    if out is not None and (out.dims != q.dims or out.dtype != "f32"):
+        raise TypeError(f"dequantize: cannot write {q!r} into {out!r}")
+    out = out if out is not None else Tensor.empty(*q.dims)
+    if lib().cleave_cuda_dequantize_e4m3(out._h, q._h, q.scales._h, *q.dims, BLOCKS[q.blocks]) != 0:
+        raise_last_error("dequantize")
+    return out
+
+
+def gemm_q_into(c: Tensor, a: QTensor, b: QTensor, *, trans_a=False, trans_b=False, bias: Tensor | None = None,
+                act: str = "identity") -> Tensor:
+    """Product of two 8-bit tensors written into the f32 matrix ``c`` (``cleave_cuda_gemm_e4m3``): ``act(op(a) @ op(b) + bias)``.
+    Shapes follow the stored layouts as in ``gemm_into``.  An operand's blocks run along the contraction or are tiles:
+    ``a`` rows (cols if ``trans_a``), ``b`` cols (rows if ``trans_b``)."""
+    if not isinstance(a, QTensor) or not isinstance(b, QTensor):
+        raise TypeError(f"gemm_q_into: operands are 8-bit tensors, got {a!r} and {b!r}")
+    m, k = (a.dims[1], a.dims[0]) if trans_a else a.dims
+    k2, n = (b.dims[1], b.dims[0]) if trans_b else b.dims
+    if k != k2 or tuple(c.dims) != (m, n):
+        raise TypeError(f"gemm_q_into: shapes {a.dims}, {b.dims} -> {c.dims} do not agree")
+    if a.blocks == ("rows" if trans_a else "cols") or b.blocks == ("cols" if trans_b else "rows"):
+        raise TypeError(f"gemm_q_into: blocks have to run along the contraction: {a!r} (trans_a={bool(trans_a)}), "
+                        f"{b!r} (trans_b={bool(trans_b)})")
+    if bias is not None and bias.dims != (n,):
+        raise TypeError(f"gemm_q_into: bias {bias!r} for {n} columns")
+    if lib().cleave_cuda_gemm_e4m3(c._h, a._h, a.scales._h, BLOCKS[a.blocks], b._h, b.scales._h, BLOCKS[b.blocks], m, n, k,
+                                   int(trans_a), int(trans_b), bias._h if bias is not None else None, ACT[act]) != 0:
+        raise_last_error("gemm_q_into")
+    return c
+
+
+def matmul_q(a: QTensor, b: QTensor) -> Tensor:
+    """``a @ b`` of 8-bit tensors as a new f32 tensor: ``a`` in rows or tiles, ``b`` in cols or tiles."""
+    return gemm_q_into(Tensor.empty(a.dims[0], b.dims[1]), a, b)

@@ -12,7 +12,7 @@ from __future__ import annotations
 import math
 
 from ._lib import lib, raise_last_error
-from .linalg import ACT, Tensor
+from .linalg import ACT, BLOCKS, QTensor, Tensor, _q_handles, _q_outputs
 
 
 def _unary(what: str):
@@ -59,6 +59,25 @@ def _bwd(fn_name: str, what: str):
 tanh_bwd = _bwd("cleave_cuda_tanh_bwd_f32", "tanh_bwd")          # (1 - y*y) * g, y = tanh(x)
 sigmoid_bwd = _bwd("cleave_cuda_sigmoid_bwd_f32", "sigmoid_bwd")  # y*(1-y) * g, y = sigmoid(x)
 relu_bwd = _bwd("cleave_cuda_relu_bwd_f32", "relu_bwd")          # x > 0 ? g : 0
+
+
+def act_bwd_q(y: QTensor, g: Tensor, act: str, *outs: QTensor, dz: Tensor | None = None, db: Tensor | None = None) -> None:
+    """Backward pass through an activation whose output ``y`` was kept as an 8-bit checkpoint: ``dz = act'(y) * g``
+    (``cleave_cuda_act_bwd_e4m3``), written in one pass into whatever is given -- ``dz`` in f32, ``outs`` in 8 bits
+    (``"rows"`` for ``dz W^T``, ``"cols"`` for ``x^T dz``) and the column sums ``db``."""
+    if not isinstance(y, QTensor) or g.dims != y.dims or g.dtype != "f32":
+        raise TypeError(f"act_bwd_q: mismatched types {y!r} and {g!r}")
+    if act not in ACT:
+        raise TypeError(f"act_bwd_q: unknown activation {act!r}")
+    if dz is not None and (dz.dims != y.dims or dz.dtype != "f32") or db is not None and (db.dims != y.dims[1:] or db.dtype != "f32"):
+        raise TypeError(f"act_bwd_q: cannot write dz {dz!r}, db {db!r} for {y!r}")
+    got = _q_outputs("act_bwd_q", y.dims, outs, ("rows", "cols"))
+    if not got and dz is None and db is None:
+        raise TypeError("act_bwd_q: no output given")
+    h = lambda t: t._h if t is not None else None  # noqa: E731
+    if lib().cleave_cuda_act_bwd_e4m3(y._h, y.scales._h, BLOCKS[y.blocks], g._h, *y.dims, ACT[act], h(dz),
+                                      *_q_handles(got, "rows"), *_q_handles(got, "cols"), h(db)) != 0:
+        raise_last_error("act_bwd_q")
 
 
 def colsum(x: Tensor) -> Tensor:

@@ -355,6 +355,49 @@ cleave_buf cleave_cuda_colsum_f64(cleave_buf x, int32_t rows, int32_t cols);
 double cleave_cuda_mse_f64(cleave_buf p, cleave_buf t, cleave_buf dp);      /* dp may be NULL */
 int32_t cleave_cuda_sgd_f64(cleave_buf w, cleave_buf g, double lr, double gscale);
 
+/* ------------------------------------------------------------------ 8-bit tensors with a scale per block of 128
+ * No counterpart in the reference (its tensors are Tensor<T: Float>, stdlib/linalg/tensor.cleave:40); they stand beside the
+ * f32 product, activations and dense-layer gradients above, for programs whose layers can run in 8 bits.
+ *
+ * A matrix [rows, cols] is two handles: e4m3 bytes (sign, 4 exponent bits, 3 mantissa bits, largest value 448, no infinity),
+ * row-major with a row pitch of cols rounded up to 16 bytes (padding bytes are never interpreted), and one f32 scale per
+ * block.  The value of an element is byte * scale.  Block forms:
+ *   ROWS    1 x 128     scales [ceil(cols/128)][rows]            an operand whose contraction runs along a row
+ *   COLS    128 x 1     scales [ceil(rows/128)][cols]            an operand whose contraction runs down a column
+ *   TILES   128 x 128   scales [ceil(rows/128)][ceil(cols/128)]  weights: either way
+ * Blocks at the right and lower edge are what is left of the matrix. */
+enum { CLEAVE_BLOCKS_ROWS = 1, CLEAVE_BLOCKS_COLS = 2, CLEAVE_BLOCKS_TILES = 3 };
+int64_t cleave_cuda_e4m3_bytes(int32_t rows, int32_t cols);                     /* length of the byte handle */
+int64_t cleave_cuda_e4m3_scales(int32_t rows, int32_t cols, int32_t blocks);    /* length of the scale handle */
+cleave_buf cleave_cuda_alloc_e4m3(int64_t bytes);                               /* uninitialised */
+cleave_buf cleave_cuda_wrap_e4m3(void* device_ptr, int64_t bytes);              /* view of caller memory, 16-byte aligned */
+cleave_buf cleave_cuda_upload_e4m3(const uint8_t* host, int64_t bytes);
+int64_t cleave_cuda_download_e4m3(cleave_buf t, uint8_t* host, int64_t bytes);  /* returns bytes or <0 */
+/* Quantizes x[rows, cols] into any of the three forms from one read of x (a form's two handles NULL: not wanted; at least
+ * one form).  Scale of a block: the smallest power of two, at least 2^-126, that brings its largest finite magnitude to at
+ * most 448; bytes: x / scale rounded to nearest, ties to even.  Non-finite values become NaN and do not count for the scale.
+ * Outputs may not share memory with each other or with x. */
+int32_t cleave_cuda_quantize_e4m3(cleave_buf x, int32_t rows, int32_t cols, cleave_buf q_rows, cleave_buf s_rows,
+                                  cleave_buf q_cols, cleave_buf s_cols, cleave_buf q_tiles, cleave_buf s_tiles);
+/* out[rows, cols] = byte * scale, rounded once (exact when the scale is a power of two). */
+int32_t cleave_cuda_dequantize_e4m3(cleave_buf out, cleave_buf q, cleave_buf s, int32_t rows, int32_t cols, int32_t blocks);
+/* c[m, n] = act(op(A) * op(B) + bias), all sums in f32.  Stored layouts as in cleave_cuda_gemm_ex_f32: A [m,k] ([k,m] if
+ * trans_a), B [k,n] ([n,k] if trans_b).  Blocks run along the contraction or are tiles: A ROWS (COLS if trans_a) or TILES,
+ * B COLS (ROWS if trans_b) or TILES; scales may be any finite f32 values.  bias may be NULL (n elements otherwise).  Any
+ * size from 1 up.  A layer's products: X W (X ROWS, W TILES), dZ W^T (dZ ROWS, W TILES, trans_b), X^T dZ (both COLS,
+ * trans_a).  The result is reproducible run to run. */
+int32_t cleave_cuda_gemm_e4m3(cleave_buf c, cleave_buf a, cleave_buf a_scale, int32_t a_blocks, cleave_buf b,
+                              cleave_buf b_scale, int32_t b_blocks, int32_t m, int32_t n, int32_t k, int32_t trans_a,
+                              int32_t trans_b, cleave_buf bias, int32_t act);
+/* Backward pass through an activation whose output y[rows, cols] was kept as an 8-bit checkpoint:
+ *   dz = act'(y) * g   with act' taken from y as in cleave_cuda_tanh_bwd_f32 / sigmoid_bwd / relu (y > 0 ? g : 0); identity: g.
+ * Writes any of: dz (f32), dz quantized into ROWS blocks (for dz W^T) and COLS blocks (for x^T dz), db = column sums of
+ * dz; NULL: not wanted, at least one.  y may have any block form.  Outputs may not share memory with each other or with
+ * y and g. */
+int32_t cleave_cuda_act_bwd_e4m3(cleave_buf y, cleave_buf y_scale, int32_t y_blocks, cleave_buf g, int32_t rows, int32_t cols,
+                                 int32_t act, cleave_buf dz, cleave_buf q_rows, cleave_buf s_rows, cleave_buf q_cols,
+                                 cleave_buf s_cols, cleave_buf db);
+
 /* ------------------------------------------------------------------ data-parallel step over peer memory
  * No counterpart in the reference (distribution is "named as a goal but not designed",
  * doc/hld.md:250).  One kernel per step does what a gradient all-reduce followed by the SGD update
