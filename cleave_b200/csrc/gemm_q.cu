@@ -20,8 +20,16 @@ namespace cleave {
 
 constexpr int kQStageP = 128 * 128;          // bytes of a P box: 128 rows (or columns) x one k-block
 constexpr int kQMaxStages = 8;
-constexpr int kQRingBudget = 104 * 1024;     // two CTAs fit an SM
+constexpr int kQRingBudget = 96 * 1024;      // two CTAs fit an SM
 constexpr int kQMaxSplit = 8;                // portable cluster size
+
+// Where a side's scales are.
+struct QScales {
+  // scale of element i of a side in k-block kb: s[kb * s_k + i * s_i + (i / 128) * s_b]
+  const float* s;
+  int64_t s_k, s_b;
+  int s_i, dim;
+};
 
 struct QGemmParams {
   float* c;
@@ -33,35 +41,37 @@ struct QGemmParams {
   int p_tiles;
   int p_mn, q_mn;         // stored with the contraction index as the row
   int swap;               // P is B (columns of C), Q is A (rows of C)
-  // scale of element i of a side in k-block kb: s[kb * s_k + i * s_i + (i / 128) * s_b]
-  const float *sp, *sq;
-  int64_t sp_k, sq_k;
-  int sp_i, sq_i;
-  int64_t sp_b, sq_b;
+  QScales sp, sq;
   int stages;
   uint32_t stage_bytes;
   DeviceStatus* status;
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
+// Bounded wait as mbar_wait, for a pipeline whose steps take a few hundred clocks: the timer, which takes as long to read as
+// such a step, is first looked at after a thousand polls.
+__device__ __forceinline__ bool q_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  unsigned long long t0 = 0;
+  for (uint32_t polls = 1;; ++polls) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((polls & 0x3FFu) == 0) {
+      if (*abort_flag) return false;
+      const unsigned long long now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > kWaitLimitNs) {
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
 }
 __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ float load_cluster_f32(uint32_t smem_addr, uint32_t rank) {
-  uint32_t a;
   float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(smem_addr, rank)) : "memory");
   return v;
 }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
@@ -92,6 +102,9 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t base, int mn_major, in
   return make_smem_desc(base + (mn_major ? kk * 4096 : kk * 32), 1024u, 2u, mn_major ? 16384u : 16u);
 }
 
+// The next k-step in a descriptor's address field (units of 16 bytes).
+__device__ __forceinline__ uint64_t k_step(int mn_major) { return mn_major ? 256u : 2u; }
+
 __device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -110,6 +123,90 @@ __device__ __forceinline__ float q_epilogue(float v, int act) {
     default: return v;
   }
 }
+
+// Arrival on a barrier of another CTA without the release of this thread's earlier writes: what it announces is that TMEM
+// loads have completed (tcgen05.wait::ld), there is no memory to publish.  The releasing form waits for the warp's
+// outstanding traffic, 1000 to 1300 clocks here, twice what a k-block's MMAs take (8192^3: 1.02 ms against 0.6).
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// Two f32 in one 64-bit register, added and multiplied lane by lane (round to nearest).
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// Waits for all TMEM loads of the warp; the registers pass through so that no use of them moves above the wait.
+__device__ __forceinline__ void tmem_wait_16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
+
+// ---- scales ----------------------------------------------------------------------------------------------------------
+// A k-block's scales come from global memory like its bytes do, a thousand clocks and more behind the request, so they are
+// fetched as far ahead: the producer warp copies them (cp.async, 4 bytes a lane: rows of scales start at any multiple of 4)
+// into a slot of their own ring, whose barrier the drain warps look at when the k-block is summed.  A slot more than the
+// k-blocks that can be under way -- the byte ring, two accumulators, one being drained -- makes every slot free when it
+// is filled again, so the ring needs no second barrier.
+__device__ __forceinline__ const float* scale_at(const QScales& o, int i) {
+  if (i >= o.dim) i = o.dim - 1;   // an element outside C: any scale will do
+  return o.s + (int64_t)i * o.s_i + (int64_t)(i >> 7) * o.s_b;
+}
+__device__ __forceinline__ void copy_scale(uint32_t dst, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// This lane's copies so far count as one arrival on `bar` once they have landed.
+__device__ __forceinline__ void arrive_after_copies(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// ---- drain ----------------------------------------------------------------------------------------------------------
+// sum += scale_p * scale_q * (this lane's row of an accumulator, COLS columns from taddr on), two sums an instruction, the next
+// 16 columns on their way from TMEM meanwhile.  scale_q: one value, or (QVEC) COLS of them, read as broadcasts.  release()
+// runs when the last columns are in registers: the accumulator is free.
+template <int COLS, bool QVEC, class Release>
+__device__ __forceinline__ void drain_columns(uint64_t (&sum)[COLS / 2], uint32_t taddr, float scale_p, const float* scale_q,
+                                              Release release) {
+  const float both = QVEC ? scale_p : __fmul_rn(scale_p, *scale_q);
+  const uint64_t both2 = pack2(__float_as_uint(both), __float_as_uint(both));
+  uint32_t r[2][16];
+  tmem_ld_16(taddr, r[0]);
+#pragma unroll
+  for (int g = 0; g < COLS / 16; ++g) {
+    tmem_wait_16(r[g & 1]);
+    if (g + 1 < COLS / 16) tmem_ld_16(taddr + (g + 1) * 16, r[(g + 1) & 1]);
+    else release();
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const uint64_t v0 = pack2(r[g & 1][2 * j], r[g & 1][2 * j + 1]);
+      const uint64_t v1 = pack2(r[g & 1][2 * j + 2], r[g & 1][2 * j + 3]);
+      if constexpr (QVEC) {
+        const ulonglong2 s = reinterpret_cast<const ulonglong2*>(scale_q)[g * 4 + j / 2];
+        sum[g * 8 + j] = fma2(mul2(v0, both2), s.x, sum[g * 8 + j]);
+        sum[g * 8 + j + 1] = fma2(mul2(v1, both2), s.y, sum[g * 8 + j + 1]);
+      } else {
+        sum[g * 8 + j] = fma2(v0, both2, sum[g * 8 + j]);
+        sum[g * 8 + j + 1] = fma2(v1, both2, sum[g * 8 + j + 1]);
+      }
+    }
+  }
+}
+__device__ __forceinline__ float low_half(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float high_half(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 
 // Columns a drain warp reads: two warps share a TMEM lane quarter from N = 64 on.
 template <int BNQ>
@@ -132,12 +229,15 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
   __shared__ __align__(8) uint64_t bar_empty[kQMaxStages];
   __shared__ __align__(8) uint64_t bar_tmem_full[2];
   __shared__ __align__(8) uint64_t bar_tmem_empty[2];
-  __shared__ __align__(16) float s_scale[T::kDrainWarps][T::kCols];
+  constexpr int kScaleQ = QVEC ? BNQ : 4;
+  __shared__ __align__(8) uint64_t bar_scale[kQMaxStages + 3];
+  __shared__ __align__(16) float scale_p[kQMaxStages + 3][128];
+  __shared__ __align__(16) float scale_q[kQMaxStages + 3][kScaleQ];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank(), ranks = cluster_size();
+  const uint32_t rank = cluster_ctarank(), ranks = cluster_size();
   const int tile = blockIdx.x / ranks;
   const int pt = tile % p.p_tiles, qt = tile / p.p_tiles;
   const int kb0 = (int)((int64_t)p.num_kb * rank / ranks), kb1 = (int)((int64_t)p.num_kb * (rank + 1) / ranks);
@@ -149,6 +249,7 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
       mbar_init(smem_u32(&bar_full[s]), 1);
       mbar_init(smem_u32(&bar_empty[s]), 1);
     }
+    for (int s = 0; s < kQMaxStages + 3; ++s) mbar_init(smem_u32(&bar_scale[s]), 32);
     for (int a = 0; a < 2; ++a) {
       mbar_init(smem_u32(&bar_tmem_full[a]), 1);
       mbar_init(smem_u32(&bar_tmem_empty[a]), T::kDrainWarps);
@@ -169,57 +270,78 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
   float* red = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)));   // the ring, once it is drained
   constexpr int kRedPitch = BNQ + 1;
 
+  const int slots = p.stages + 3;
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0, issued = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag)) {
-          report(p.status, 1, 1100 + stage, kb);
-          ok = false;
-          break;
-        }
+    int stage = 0, slot = 0, issued = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const float* src_p[4];
+    constexpr int kPerQ = QVEC ? (BNQ + 31) / 32 : 1;
+    const float* src_q[kPerQ];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) src_p[i] = scale_at(p.sp, pt * 128 + lane + 32 * i) + (int64_t)kb0 * p.sp.s_k;
+#pragma unroll
+    for (int i = 0; i < kPerQ; ++i) src_q[i] = scale_at(p.sq, qt * BNQ + (QVEC ? lane + 32 * i : 0)) + (int64_t)kb0 * p.sq.s_k;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      ok = __all_sync(0xffffffffu, q_wait(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag));
+      if (!ok) {
+        if (lane == 0) report(p.status, 1, 1100 + stage, kb);
+        break;
+      }
+      if (lane == 0) {
         const uint32_t full = smem_u32(&bar_full[stage]);
         mbar_arrive_expect_tx(full, p.stage_bytes);
         const uint32_t sp = ring + stage * p.stage_bytes;
-        if (p.p_mn) tma_load_2d(sp, &map_p, full, pt * 128, kb * 128);
-        else tma_load_2d(sp, &map_p, full, kb * 128, pt * 128);
-        if (p.q_mn) tma_load_2d(sp + kQStageP, &map_q, full, qt * BNQ, kb * 128);
-        else tma_load_2d(sp + kQStageP, &map_q, full, kb * 128, qt * BNQ);
-        ++issued;
-        if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+        tma_load_2d(sp, &map_p, full, p.p_mn ? pt * 128 : kb * 128, p.p_mn ? kb * 128 : pt * 128);
+        tma_load_2d(sp + kQStageP, &map_q, full, p.q_mn ? qt * BNQ : kb * 128, p.q_mn ? kb * 128 : qt * BNQ);
       }
-      if (!ok) {
-        // leaving early: give the copies in flight a bounded chance to land
-        for (int s = 0; s < p.stages; ++s) {
-          const int fills = (issued + p.stages - 1 - s) / p.stages;   // how often stage s was filled
-          if (fills == 0) continue;
-          for (int spin = 0; spin < (1 << 20); ++spin)
-            if (mbar_try_wait(smem_u32(&bar_full[s]), (uint32_t)(fills - 1) & 1u)) break;
-        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        copy_scale(smem_u32(&scale_p[slot][lane + 32 * i]), src_p[i]);
+        src_p[i] += p.sp.s_k;
+      }
+#pragma unroll
+      for (int i = 0; i < kPerQ; ++i) {
+        if (lane + 32 * i < kScaleQ) copy_scale(smem_u32(&scale_q[slot][lane + 32 * i]), src_q[i]);
+        src_q[i] += p.sq.s_k;
+      }
+      arrive_after_copies(smem_u32(&bar_scale[slot]));
+      ++issued;
+      if (++slot == slots) slot = 0;
+      if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+    }
+    if (!ok) {
+      // leaving early: give the copies in flight a bounded chance to land
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      for (int s = 0; lane == 0 && s < p.stages; ++s) {
+        const int fills = (issued + p.stages - 1 - s) / p.stages;   // how often stage s was filled
+        if (fills == 0) continue;
+        for (int spin = 0; spin < (1 << 20); ++spin)
+          if (mbar_try_wait(smem_u32(&bar_full[s]), (uint32_t)(fills - 1) & 1u)) break;
       }
     }
   } else if (warp == 1) {
     if (lane == 0) {
       const uint32_t idesc = instr_desc_e4m3(p.p_mn, p.q_mn, 128, BNQ);
+      const uint64_t desc_p = operand_desc(ring, p.p_mn, 0), desc_q = operand_desc(ring + kQStageP, p.q_mn, 0);
+      const uint64_t step_p = k_step(p.p_mn), step_q = k_step(p.q_mn);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(smem_u32(&bar_tmem_empty[acc]), acc_phase ^ 1u, &abort_flag)) {
+        if (!q_wait(smem_u32(&bar_tmem_empty[acc]), acc_phase ^ 1u, &abort_flag)) {
           report(p.status, 2, 1200 + acc, kb);
           break;
         }
-        if (!mbar_wait(smem_u32(&bar_full[stage]), phase, &abort_flag)) {
+        if (!q_wait(smem_u32(&bar_full[stage]), phase, &abort_flag)) {
           report(p.status, 3, 1300 + stage, kb);
           break;
         }
         tcgen05_fence_after();
-        const uint32_t sp = ring + stage * p.stage_bytes;
+        const uint64_t at = (uint64_t)(stage * p.stage_bytes) >> 4;
         const uint32_t d = tmem_base + (uint32_t)(acc * BNQ);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          umma_e4m3(d, operand_desc(sp, p.p_mn, kk), operand_desc(sp + kQStageP, p.q_mn, kk), idesc, kk ? 1u : 0u);
+          umma_e4m3(d, desc_p + at + kk * step_p, desc_q + at + kk * step_q, idesc, kk ? 1u : 0u);
         tcgen05_commit(smem_u32(&bar_empty[stage]));
         tcgen05_commit(smem_u32(&bar_tmem_full[acc]));
         if (++stage == p.stages) { stage = 0; phase ^= 1u; }
@@ -227,43 +349,15 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
       }
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2, dw = warp - 2;
-    int pi = pt * 128 + quarter * 32 + lane;
-    if (pi >= p.p_dim) pi = p.p_dim - 1;   // a row outside C: any scale will do
-    const float* sp = p.sp + (int64_t)pi * p.sp_i + (int64_t)(pi >> 7) * p.sp_b;
-    const int q0 = qt * BNQ + half * T::kCols;
-    constexpr int kPer = QVEC ? (T::kCols + 31) / 32 : 1;
-    const float* sq[kPer];
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    uint64_t sum[T::kCols / 2];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      int qi = QVEC ? q0 + lane + 32 * i : q0;
-      if (qi >= p.q_dim) qi = p.q_dim - 1;
-      sq[i] = p.sq + (int64_t)qi * p.sq_i + (int64_t)(qi >> 7) * p.sq_b;
-    }
-    float acc_sum[T::kCols];
-#pragma unroll
-    for (int j = 0; j < T::kCols; ++j) acc_sum[j] = 0.0f;
-    float next_p = __ldg(sp + (int64_t)kb0 * p.sp_k), next_q[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) next_q[i] = __ldg(sq[i] + (int64_t)kb0 * p.sq_k);
-    int acc = 0;
-    uint32_t acc_phase = 0;
+    for (int j = 0; j < T::kCols / 2; ++j) sum[j] = 0;
+    int acc = 0, slot = 0;
+    uint32_t acc_phase = 0, slot_phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
-      const float cur_p = next_p;
-      float cur_q = next_q[0];
-      if constexpr (QVEC) {
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if (lane + 32 * i < T::kCols) s_scale[dw][lane + 32 * i] = next_q[i];
-        __syncwarp();
-      }
-      if (kb + 1 < kb1) {   // the next block's scales travel while this one is drained
-        next_p = __ldg(sp + (int64_t)(kb + 1) * p.sp_k);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) next_q[i] = __ldg(sq[i] + (int64_t)(kb + 1) * p.sq_k);
-      }
-      bool ok = mbar_wait(smem_u32(&bar_tmem_full[acc]), acc_phase, &abort_flag);
+      bool ok = q_wait(smem_u32(&bar_scale[slot]), slot_phase, &abort_flag) &&
+                q_wait(smem_u32(&bar_tmem_full[acc]), acc_phase, &abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
         if (lane == 0) report(p.status, 4, 1400 + acc, kb);
@@ -271,35 +365,27 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
       }
       tcgen05_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BNQ + half * T::kCols);
-      const float both = __fmul_rn(cur_p, cur_q);
-#pragma unroll
-      for (int g = 0; g < T::kCols / 16; ++g) {
-        uint32_t r[16];
-        tmem_ld_16(taddr + g * 16, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if constexpr (QVEC)
-            acc_sum[g * 16 + j] = __fmaf_rn(__fmul_rn(__uint_as_float(r[j]), cur_p), s_scale[dw][g * 16 + j], acc_sum[g * 16 + j]);
-          else
-            acc_sum[g * 16 + j] = __fmaf_rn(__uint_as_float(r[j]), both, acc_sum[g * 16 + j]);
-        }
-      }
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_tmem_empty[acc]));
+      drain_columns<T::kCols, QVEC>(sum, taddr, scale_p[slot][quarter * 32 + lane], &scale_q[slot][QVEC ? half * T::kCols : 0], [&] {
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_tmem_empty[acc]));
+      });
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      if (++slot == slots) { slot = 0; slot_phase ^= 1u; }
     }
     // Every load has landed and every MMA has read it: the ring is free for the partial sums.
 #pragma unroll
-    for (int j = 0; j < T::kCols; ++j)
-      red[(quarter * 32 + lane) * kRedPitch + half * T::kCols + j] = acc_sum[j];
+    for (int j = 0; j < T::kCols / 2; ++j) {
+      float* at = red + (quarter * 32 + lane) * kRedPitch + half * T::kCols + 2 * j;
+      at[0] = low_half(sum[j]);
+      at[1] = high_half(sum[j]);
+    }
   }
 
   __syncwarp();
   tcgen05_fence_before();
   __syncthreads();
-  if (ranks > 1) cluster_barrier();
+  if (ranks > 1) cluster_sync_all();
   if (!abort_flag) {
     // This CTA's share of the tile's P rows, summed over the ranks in ascending order and stored along C's rows.
     const int share = 128 / (int)ranks, first = (int)rank * share;
@@ -323,11 +409,311 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
   }
   if (ranks > 1) {
     __syncwarp();
-    cluster_barrier();   // the peers are done with this CTA's shared memory
+    cluster_sync_all();   // the peers are done with this CTA's shared memory
   }
   if (warp == 1) {
     tcgen05_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)T::kTmem) : "memory");
+  }
+}
+
+// ---- large products: CTA pairs ---------------------------------------------------------------------------------------
+// The two CTAs of a cluster share a 256 x 256 tile (tcgen05 cta_group::2): each stages 128 rows of P and 128 of Q per
+// k-block (32 KiB a stage, five stages), the MMA of CTA 0 reads Q from both, each CTA drains the sums of its own 128 rows.
+// Persistent over the tiles; barriers as in gemm_tc_pair.cu.  At the tensor pipe's rate a k-block takes 512 clocks, in
+// which the eight drain warps read 128 x 256 sums from TMEM and add them, scaled, to 128 running sums a thread.
+constexpr int kQPairStages = 5;
+constexpr int kQPairSlots = kQPairStages + 3;
+constexpr int kQPairStageBytes = 2 * kQStageP;
+constexpr int kQPairRing = kQPairStages * kQPairStageBytes;
+constexpr int kQPairSmem = kQPairRing + kEpiWarps * 32 * 128 + 1024;
+
+struct QPairParams {
+  TcParams t;             // c, bias, act, m, n, num_kb, mblks, nblks, pair_group_m, c_tma, status
+  int p_mn, q_mn;
+  QScales sp, sq;
+};
+
+__device__ __forceinline__ void tma_pair_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar_cluster, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar_cluster), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void umma_e4m3_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Adds the bias, applies the activation and stores a drain warp's 32 x 32 block of C whose first element is (row0, col0);
+// lane r holds row r.  The block passes through the warp's staging tile (16-byte word j of row r at slot j ^ (r & 7):
+// conflict free, and TMA's 128-byte swizzle) and leaves as one bulk tensor store, which clips what lies outside C, or, where
+// no tensor map describes C, as 128-byte rows.
+__device__ __forceinline__ void store_q_block(float (&v)[32], const TcParams& p, const CUtensorMap* map_c, float4* stage,
+                                              int row0, int col0, int lane) {
+  if (row0 >= p.m || col0 >= p.n) return;   // uniform over the warp
+  if (p.bias != nullptr) {
+    if (col0 + 32 <= p.n && (reinterpret_cast<uintptr_t>(p.bias + col0) & 15u) == 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + col0) + j);
+        v[4 * j] = __fadd_rn(v[4 * j], b.x);
+        v[4 * j + 1] = __fadd_rn(v[4 * j + 1], b.y);
+        v[4 * j + 2] = __fadd_rn(v[4 * j + 2], b.z);
+        v[4 * j + 3] = __fadd_rn(v[4 * j + 3], b.w);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (col0 + j < p.n) v[j] = __fadd_rn(v[j], __ldg(p.bias + col0 + j));
+    }
+  }
+  if (p.act == CLEAVE_ACT_TANH) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = q_epilogue(v[j], CLEAVE_ACT_TANH);
+  } else if (p.act == CLEAVE_ACT_SIGMOID) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = q_epilogue(v[j], CLEAVE_ACT_SIGMOID);
+  } else if (p.act == CLEAVE_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = q_epilogue(v[j], CLEAVE_ACT_RELU);
+  }
+  if (p.c_tma) {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the tile's last store has been read
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      stage[lane * 8 + (j ^ (lane & 7))] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // generic writes -> visible to the copy engine
+    __syncwarp();
+    if (lane == 0) {
+      asm volatile(
+          "cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+          ::"l"(map_c), "r"(smem_u32(stage)), "r"(col0), "r"(row0), "r"(0)
+          : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+    return;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    stage[lane * 8 + (j ^ (lane & 7))] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  __syncwarp();
+  const float* words = reinterpret_cast<const float*>(stage);
+  const int rows = p.m - row0 < 32 ? p.m - row0 : 32;
+  if (col0 + lane < p.n) {
+    float* dst = p.c + (int64_t)row0 * p.n + col0 + lane;
+    for (int r = 0; r < rows; ++r) dst[(int64_t)r * p.n] = words[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)];
+  }
+}
+
+__device__ __forceinline__ void decode_q_tile(int t, const TcParams& p, int& mb, int& nb) {
+  const int span = p.pair_group_m * p.nblks;
+  const int first = t / span * p.pair_group_m;
+  const int rows_here = (p.mblks - first) < p.pair_group_m ? (p.mblks - first) : p.pair_group_m;
+  const int r = t % span;
+  mb = first + r % rows_here;
+  nb = r / rows_here;
+}
+
+template <bool QVEC>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+gemm_q_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                   const __grid_constant__ CUtensorMap map_c, const QPairParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bar_full[kQPairStages];
+  __shared__ __align__(8) uint64_t bar_empty[kQPairStages];
+  __shared__ __align__(8) uint64_t bar_tmem_full[kAccStages];
+  __shared__ __align__(8) uint64_t bar_tmem_empty[kAccStages];
+  constexpr int kScaleQ = QVEC ? 256 : 4;   // one value for each 128 columns, or one for every column
+  __shared__ __align__(8) uint64_t bar_scale[kQPairSlots];
+  __shared__ __align__(16) float scale_p[kQPairSlots][128];
+  __shared__ __align__(16) float scale_q[kQPairSlots][kScaleQ];
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const int tiles = p.t.mblks * p.t.nblks, n_clusters = gridDim.x >> 1, num_kb = p.t.num_kb;
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < kQPairStages; ++s) {
+      mbar_init(smem_u32(&bar_full[s]), 1);
+      mbar_init(smem_u32(&bar_empty[s]), 1);
+    }
+    for (int s = 0; s < kQPairSlots; ++s) mbar_init(smem_u32(&bar_scale[s]), 32);
+    for (int a = 0; a < kAccStages; ++a) {
+      mbar_init(smem_u32(&bar_tmem_full[a]), 1);
+      mbar_init(smem_u32(&bar_tmem_empty[a]), 2 * kEpiWarps);   // the drain warps of both CTAs
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                 "r"((uint32_t)kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();   // both CTAs' barriers and TMEM exist before anything crosses over
+  tcgen05_fence_after();
+  const uint32_t tmem_base = tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_p) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
+    }
+    int stage = 0, slot = 0, issued = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int t = blockIdx.x >> 1; ok && t < tiles; t += n_clusters) {
+      int mb, nb;
+      decode_q_tile(t, p.t, mb, nb);
+      const int p0 = mb * 256 + (int)rank * 128, q0 = nb * 256 + (int)rank * 128;
+      const float* src_p[4];
+      constexpr int kPerQ = QVEC ? 8 : 1;
+      const float* src_q[kPerQ];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) src_p[i] = scale_at(p.sp, p0 + lane + 32 * i);
+#pragma unroll
+      for (int i = 0; i < kPerQ; ++i) src_q[i] = scale_at(p.sq, nb * 256 + (QVEC ? lane + 32 * i : (lane & 1) * 128));
+      for (int kb = 0; kb < num_kb; ++kb) {
+        ok = __all_sync(0xffffffffu, q_wait(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag));
+        if (!ok) {
+          if (lane == 0) report(p.t.status, 1, 1500 + stage, kb);
+          break;
+        }
+        if (lane == 0) {
+          const uint32_t full_own = smem_u32(&bar_full[stage]);
+          const uint32_t full0 = map_to_cta(full_own, 0);
+          if (rank == 0) mbar_arrive_expect_tx(full_own, 2 * kQPairStageBytes);   // both CTAs' boxes
+          const uint32_t sp = ring + stage * kQPairStageBytes;
+          tma_pair_load_2d(sp, &map_p, full0, p.p_mn ? p0 : kb * 128, p.p_mn ? kb * 128 : p0);
+          tma_pair_load_2d(sp + kQStageP, &map_q, full0, p.q_mn ? q0 : kb * 128, p.q_mn ? kb * 128 : q0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          copy_scale(smem_u32(&scale_p[slot][lane + 32 * i]), src_p[i]);
+          src_p[i] += p.sp.s_k;
+        }
+#pragma unroll
+        for (int i = 0; i < kPerQ; ++i) {
+          if (lane + 32 * i < kScaleQ) copy_scale(smem_u32(&scale_q[slot][lane + 32 * i]), src_q[i]);
+          src_q[i] += p.sq.s_k;
+        }
+        arrive_after_copies(smem_u32(&bar_scale[slot]));
+        ++issued;
+        if (++slot == kQPairSlots) slot = 0;
+        if (++stage == kQPairStages) { stage = 0; phase ^= 1u; }
+      }
+    }
+    if (!ok) {
+      // leaving early: give the copies in flight a bounded chance to land (CTA 0 sees their completion)
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      for (int s = 0; rank == 0 && lane == 0 && s < kQPairStages; ++s) {
+        const int fills = (issued + kQPairStages - 1 - s) / kQPairStages;
+        if (fills == 0) continue;
+        for (int spin = 0; spin < (1 << 20); ++spin)
+          if (mbar_try_wait(smem_u32(&bar_full[s]), (uint32_t)(fills - 1) & 1u)) break;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = instr_desc_e4m3(p.p_mn, p.q_mn, 256, 256);
+      const uint64_t desc_p = operand_desc(ring, p.p_mn, 0), desc_q = operand_desc(ring + kQStageP, p.q_mn, 0);
+      const uint64_t step_p = k_step(p.p_mn), step_q = k_step(p.q_mn);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x >> 1; ok && t < tiles; t += n_clusters) {
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!q_wait(smem_u32(&bar_tmem_empty[acc]), acc_phase ^ 1u, &abort_flag)) {
+            report(p.t.status, 2, 1600 + acc, kb);
+            ok = false;
+            break;
+          }
+          if (!q_wait(smem_u32(&bar_full[stage]), phase, &abort_flag)) {
+            report(p.t.status, 3, 1700 + stage, kb);
+            ok = false;
+            break;
+          }
+          tcgen05_fence_after();
+          const uint64_t at = (uint64_t)(stage * kQPairStageBytes) >> 4;
+          const uint32_t d = tmem_base + (uint32_t)(acc * BN);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_e4m3_pair(d, desc_p + at + kk * step_p, desc_q + at + kk * step_q, idesc, kk ? 1u : 0u);
+          tcgen05_commit_pair(smem_u32(&bar_empty[stage]));
+          tcgen05_commit_pair(smem_u32(&bar_tmem_full[acc]));
+          if (++stage == kQPairStages) { stage = 0; phase ^= 1u; }
+          if (++acc == kAccStages) { acc = 0; acc_phase ^= 1u; }
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    int acc = 0, slot = 0;
+    uint32_t acc_phase = 0, slot_phase = 0;
+    float4* stage_tile = reinterpret_cast<float4*>(smem_raw + (ring - smem_u32(smem_raw)) + kQPairRing) + (warp - 2) * (32 * 8);
+    bool ok = true;
+    for (int t = blockIdx.x >> 1; ok && t < tiles; t += n_clusters) {
+      int mb, nb;
+      decode_q_tile(t, p.t, mb, nb);
+      uint64_t sum[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) sum[j] = 0;
+      for (int kb = 0; kb < num_kb; ++kb) {
+        ok = q_wait(smem_u32(&bar_scale[slot]), slot_phase, &abort_flag) &&
+             q_wait(smem_u32(&bar_tmem_full[acc]), acc_phase, &abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          if (lane == 0) report(p.t.status, 4, 1800 + acc, kb);
+          break;
+        }
+        tcgen05_fence_after();
+        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN + half * 128);
+        drain_columns<128, QVEC>(sum, taddr, scale_p[slot][quarter * 32 + lane], &scale_q[slot][QVEC ? half * 128 : half], [&] {
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&bar_tmem_empty[acc]), 0));
+        });
+        if (++acc == kAccStages) { acc = 0; acc_phase ^= 1u; }
+        if (++slot == kQPairSlots) { slot = 0; slot_phase ^= 1u; }
+      }
+      if (!ok) break;
+#pragma unroll
+      for (int pass = 0; pass < 4; ++pass) {
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          v[2 * j] = low_half(sum[pass * 16 + j]);
+          v[2 * j + 1] = high_half(sum[pass * 16 + j]);
+        }
+        store_q_block(v, p.t, &map_c, stage_tile, mb * 256 + (int)rank * 128 + quarter * 32, nb * 256 + half * 128 + 32 * pass,
+                      lane);
+      }
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // stores have reached memory
+  }
+
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();   // the peer can no longer issue an MMA into this CTA's TMEM or signal its barriers
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)kTmemCols)
+                 : "memory");
   }
 }
 
@@ -361,17 +747,11 @@ static bool side_map(CUtensorMap* map, const QSide& o, int box) {
   return true;
 }
 
-// Strides of a side's scales (QGemmParams).  Vector blocks run along k whichever way the operand is stored.
-static void side_scales(const QSide& o, int64_t* s_k, int* s_i, int64_t* s_b) {
-  if (o.blocks == CLEAVE_BLOCKS_TILES) {
-    *s_i = 0;
-    *s_k = o.mn ? ceil_div(o.dim, kQBlock) : 1;
-    *s_b = o.mn ? 1 : ceil_div(o.k, kQBlock);
-  } else {
-    *s_i = 1;
-    *s_k = o.dim;
-    *s_b = 0;
-  }
+// Where a side's scales are.  Vector blocks run along k whichever way the operand is stored.
+static QScales side_scales(const QSide& o) {
+  if (o.blocks != CLEAVE_BLOCKS_TILES) return {o.s, o.dim, 0, 1, o.dim};
+  if (o.mn) return {o.s, ceil_div(o.dim, kQBlock), 1, 0, o.dim};
+  return {o.s, 1, ceil_div(o.k, kQBlock), 0, o.dim};
 }
 
 template <int BNQ, bool QVEC>
@@ -404,7 +784,53 @@ static bool launch_q(const CUtensorMap& map_p, const CUtensorMap& map_q, const Q
   return ok;
 }
 
+template <bool QVEC>
+static bool launch_q_pair(const CUtensorMap* maps, const QPairParams& p) {
+  static bool attr_set = false;
+  if (!attr_set) {
+    if (!cuda_ok(cudaFuncSetAttribute(gemm_q_pair_kernel<QVEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, kQPairSmem),
+                 "cudaFuncSetAttribute(8-bit pair gemm)"))
+      return false;
+    attr_set = true;
+  }
+  const int tiles = p.t.mblks * p.t.nblks, pairs = ctx().sm_count / 2;
+  profile_mark(true);
+  gemm_q_pair_kernel<QVEC><<<2 * (tiles < pairs ? tiles : pairs), kGemmThreads, kQPairSmem, ctx().stream>>>(maps[0], maps[1],
+                                                                                                         maps[2], p);
+  count_launch();
+  const bool ok = cuda_ok(cudaGetLastError(), "8-bit pair GEMM launch");
+  profile_mark(false);
+  return ok;
+}
+
+static bool gemm_q_pairs(const QSide& a, const QSide& b, float* c, const float* bias, int act) {
+  QPairParams p = {};
+  p.t.c = c;
+  p.t.bias = bias;
+  p.t.act = act;
+  p.t.m = a.dim;
+  p.t.n = b.dim;
+  p.t.num_kb = ceil_div(a.k, kQBlock);
+  p.t.mblks = ceil_div(a.dim, 256);
+  p.t.nblks = ceil_div(b.dim, 256);
+  p.t.pair_group_m = 8;
+  p.t.status = ctx().status_dev;
+  p.p_mn = a.mn;
+  p.q_mn = b.mn;
+  p.sp = side_scales(a);
+  p.sq = side_scales(b);
+  CUtensorMap maps[3];
+  if (!side_map(&maps[0], a, 128) || !side_map(&maps[1], b, 128)) return false;
+  maps[2] = maps[0];
+  // whole 32 x 32 blocks of C leave as bulk tensor stores where a tensor map can describe C
+  p.t.c_tma = aligned16(c) && b.dim % 4 == 0 && make_c_map(&maps[2], c, a.dim, b.dim, 1, 1) ? 1 : 0;
+  return b.blocks == CLEAVE_BLOCKS_TILES ? launch_q_pair<false>(maps, p) : launch_q_pair<true>(maps, p);
+}
+
 static bool gemm_q(const QSide& a, const QSide& b, float* c, const float* bias, int act) {
+  const int64_t pair_tiles = (int64_t)ceil_div(a.dim, 256) * ceil_div(b.dim, 256);
+  if (pair_tiles >= ctx().sm_count / 4 && pair_tiles <= 0x3fffffff && a.dim > 128 && b.dim > 128)
+    return gemm_q_pairs(a, b, c, bias, act);
   QGemmParams p = {};
   p.c = c;
   p.bias = bias;
@@ -420,10 +846,8 @@ static bool gemm_q(const QSide& a, const QSide& b, float* c, const float* bias, 
   p.q_dim = Q.dim;
   p.p_mn = P.mn;
   p.q_mn = Q.mn;
-  p.sp = P.s;
-  p.sq = Q.s;
-  side_scales(P, &p.sp_k, &p.sp_i, &p.sp_b);
-  side_scales(Q, &p.sq_k, &p.sq_i, &p.sq_b);
+  p.sp = side_scales(P);
+  p.sq = side_scales(Q);
   p.status = ctx().status_dev;
   const int bn = Q.dim <= 16 ? 16 : Q.dim <= 32 ? 32 : Q.dim <= 64 ? 64 : 128;
   p.stage_bytes = kQStageP + (Q.mn ? kQStageP : bn * 128);

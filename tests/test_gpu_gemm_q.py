@@ -55,7 +55,21 @@ def test_product_every_order_and_block_form(m, n, k, ta, tb):
         assert np.all(err <= bound(av, bv)), (fa, fb, float(np.max(err / bound(av, bv))))
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 200, 300), (40, 333, 512), (150, 270, 1100), (513, 514, 515)])
+@pytest.mark.parametrize("m,n,k", [(1537, 1799, 391), (2048, 1284, 1024), (130, 9000, 128)])
+@pytest.mark.parametrize("ta,tb", TRANS)
+def test_large_product_every_order(m, n, k, ta, tb):
+    # enough 256 x 256 tiles for CTA pairs; ragged edges, a width that TMA stores can take and one that they cannot
+    for i, (fa, fb) in enumerate(forms(ta, tb)[:2]):
+        a, av = operand(31 + i, m, k, ta, fa)
+        b, bv = operand(41 + i, n, k, not tb, fb)
+        bias = np.random.default_rng(5).standard_normal(n).astype(f32)
+        c = linalg.gemm_q_into(Tensor.filled(np.nan, m, n), a, b, trans_a=bool(ta), trans_b=bool(tb), bias=Tensor(bias),
+                               act="relu").numpy()
+        z = av @ bv.T + bias
+        assert np.all(np.abs(c - np.maximum(z, 0)) <= bound(av, bv) + 2.0 ** -24 * np.abs(z))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 200, 300), (40, 333, 512), (150, 270, 1100), (513, 514, 515), (1700, 1600, 260)])
 @pytest.mark.parametrize("ta,tb", TRANS)
 def test_small_integers_are_exact(m, n, k, ta, tb):
     # integers up to 8 are e4m3 values, every partial sum is an integer below 2^24: no rounding anywhere
