@@ -47,13 +47,40 @@ struct QGemmParams {
   DeviceStatus* status;
 };
 
-// Bounded wait as mbar_wait, for a pipeline whose steps take a few hundred clocks: the timer, which takes as long to read as
-// such a step, is first looked at after a thousand polls.
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+// Bounded wait as mbar_wait, for pipelines whose steps take a few hundred clocks.  A waiting warp sleeps in the barrier (for up
+// to kSleepNs at a time, woken when the phase completes) instead of polling: with 20 warps a CTA, polls took issue slots from
+// the warps at work.  The timer, as slow to read as a step, is looked at every 16 sleeps.
+constexpr uint32_t kSleepNs = 200000;
+// CLUSTER: for a barrier through which another CTA released generic writes.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool q_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   unsigned long long t0 = 0;
-  for (uint32_t polls = 1;; ++polls) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((polls & 0x3FFu) == 0) {
+  for (uint32_t sleeps = 1;; ++sleeps) {
+    uint32_t ok;
+    if constexpr (CLUSTER)
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(bar), "r"(parity), "r"(kSleepNs)
+          : "memory");
+    else
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(bar), "r"(parity), "r"(kSleepNs)
+          : "memory");
+    if (ok) return true;
+    if ((sleeps & 15u) == 0) {
       if (*abort_flag) return false;
       const unsigned long long now = globaltimer_ns();
       if (t0 == 0) t0 = now;
@@ -115,11 +142,33 @@ __device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
       : "memory");
 }
 
+// tanh(x) = x N(x^2) / D(x^2): a rational approximation of degree 4 / 4 (relative error 2.2e-8 on [-9.02, 9.02], fitted in
+// 50 digits for the least largest error; beyond, tanh rounds to 1), one reciprocal corrected to a division.  Within 3.4e-7 of
+// the value everywhere.  tanhf takes twice the instructions, and the epilogue of a product with a short contraction is
+// bound by them (4096 x 4096, k 1024: 48 us with it, 38 without an activation).
+__device__ __forceinline__ float q_tanh(float x) {
+  const float a = fabsf(x) > 9.02f ? copysignf(9.02f, x) : x;   // a NaN stays
+  const float s = __fmul_rn(a, a);
+  float n = 1.3328731e-8f, d = 7.7662906e-7f;
+  n = __fmaf_rn(n, s, 2.0591549e-5f);
+  d = __fmaf_rn(d, s, 3.2839418e-4f);
+  n = __fmaf_rn(n, s, 3.4945765e-3f);
+  d = __fmaf_rn(d, s, 2.5873192e-2f);
+  n = __fmaf_rn(n, s, 1.3380193e-1f);
+  d = __fmaf_rn(d, s, 4.6713510e-1f);
+  n = __fmul_rn(__fmaf_rn(n, s, 1.0f), a);
+  d = __fmaf_rn(d, s, 1.0f);
+  const float r = __fdividef(1.0f, d);
+  float q = __fmul_rn(n, r);
+  q = __fmaf_rn(__fmaf_rn(-q, d, n), r, q);
+  return fabsf(q) > 1.0f ? copysignf(1.0f, q) : q;
+}
+
 __device__ __forceinline__ float q_epilogue(float v, int act) {
   switch (act) {
     case CLEAVE_ACT_RELU: return act_apply(v, CLEAVE_ACT_RELU);
     case CLEAVE_ACT_SIGMOID: return __fdividef(1.0f, 1.0f + __expf(-v));   // as the f32 product's epilogue
-    case CLEAVE_ACT_TANH: return tanhf(v);
+    case CLEAVE_ACT_TANH: return q_tanh(v);
     default: return v;
   }
 }
@@ -162,9 +211,9 @@ __device__ __forceinline__ void tmem_wait_16(uint32_t (&r)[16]) {
 // into a slot of their own ring, whose barrier the drain warps look at when the k-block is summed.  A slot more than the
 // k-blocks that can be under way -- the byte ring, two accumulators, one being drained -- makes every slot free when it
 // is filled again, so the ring needs no second barrier.
-__device__ __forceinline__ const float* scale_at(const QScales& o, int i) {
+__device__ __forceinline__ uint32_t scale_offset(const QScales& o, int i) {
   if (i >= o.dim) i = o.dim - 1;   // an element outside C: any scale will do
-  return o.s + (int64_t)i * o.s_i + (int64_t)(i >> 7) * o.s_b;
+  return (uint32_t)(i * o.s_i) + (uint32_t)((i >> 7) * o.s_b);   // below 2^31: i, or the number of tiles
 }
 __device__ __forceinline__ void copy_scale(uint32_t dst, const float* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -175,32 +224,41 @@ __device__ __forceinline__ void arrive_after_copies(uint32_t bar) {
 }
 
 // ---- drain ----------------------------------------------------------------------------------------------------------
-// sum += scale_p * scale_q * (this lane's row of an accumulator, COLS columns from taddr on), two sums an instruction, the next
-// 16 columns on their way from TMEM meanwhile.  scale_q: one value, or (QVEC) COLS of them, read as broadcasts.  release()
-// runs when the last columns are in registers: the accumulator is free.
-template <int COLS, bool QVEC, class Release>
+// sum += scale_p * scale_q * (this lane's row of an accumulator, COLS columns from taddr on), two sums an instruction.
+// scale_q: one value, or (QVEC) COLS of them, read as broadcasts.  release() runs once the last columns are in registers:
+// the accumulator is free.
+template <int PIECE>
+__device__ __forceinline__ void tmem_ld_wait_piece(uint32_t taddr, uint32_t (&r)[PIECE]) {
+  if constexpr (PIECE == 32) {
+    tmem_ld_32x32(taddr, r);
+    tmem_ld_wait_for(r);
+  } else {
+    tmem_ld_16(taddr, r);
+    tmem_wait_16(r);
+  }
+}
+template <int COLS, int PIECE, bool QVEC, class Release>
 __device__ __forceinline__ void drain_columns(uint64_t (&sum)[COLS / 2], uint32_t taddr, float scale_p, const float* scale_q,
                                               Release release) {
+  constexpr int kPiece = PIECE;
   const float both = QVEC ? scale_p : __fmul_rn(scale_p, *scale_q);
   const uint64_t both2 = pack2(__float_as_uint(both), __float_as_uint(both));
-  uint32_t r[2][16];
-  tmem_ld_16(taddr, r[0]);
 #pragma unroll
-  for (int g = 0; g < COLS / 16; ++g) {
-    tmem_wait_16(r[g & 1]);
-    if (g + 1 < COLS / 16) tmem_ld_16(taddr + (g + 1) * 16, r[(g + 1) & 1]);
-    else release();
+  for (int g = 0; g < COLS / kPiece; ++g) {
+    uint32_t r[kPiece];
+    tmem_ld_wait_piece<kPiece>(taddr + g * kPiece, r);
+    if (g == COLS / kPiece - 1) release();
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const uint64_t v0 = pack2(r[g & 1][2 * j], r[g & 1][2 * j + 1]);
-      const uint64_t v1 = pack2(r[g & 1][2 * j + 2], r[g & 1][2 * j + 3]);
+    for (int j = 0; j < kPiece / 2; j += 2) {
+      const uint64_t v0 = pack2(r[2 * j], r[2 * j + 1]), v1 = pack2(r[2 * j + 2], r[2 * j + 3]);
+      uint64_t &s0 = sum[g * kPiece / 2 + j], &s1 = sum[g * kPiece / 2 + j + 1];
       if constexpr (QVEC) {
-        const ulonglong2 s = reinterpret_cast<const ulonglong2*>(scale_q)[g * 4 + j / 2];
-        sum[g * 8 + j] = fma2(mul2(v0, both2), s.x, sum[g * 8 + j]);
-        sum[g * 8 + j + 1] = fma2(mul2(v1, both2), s.y, sum[g * 8 + j + 1]);
+        const ulonglong2 q = reinterpret_cast<const ulonglong2*>(scale_q)[g * kPiece / 4 + j / 2];
+        s0 = fma2(mul2(v0, both2), q.x, s0);
+        s1 = fma2(mul2(v1, both2), q.y, s1);
       } else {
-        sum[g * 8 + j] = fma2(v0, both2, sum[g * 8 + j]);
-        sum[g * 8 + j + 1] = fma2(v1, both2, sum[g * 8 + j + 1]);
+        s0 = fma2(v0, both2, s0);
+        s1 = fma2(v1, both2, s1);
       }
     }
   }
@@ -226,8 +284,7 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
   typedef QTile<BNQ> T;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[kQMaxStages];
-  __shared__ __align__(8) uint64_t bar_empty[kQMaxStages];
-  __shared__ __align__(8) uint64_t bar_tmem_full[2];
+  __shared__ __align__(8) uint64_t bar_done[kQMaxStages];
   __shared__ __align__(8) uint64_t bar_tmem_empty[2];
   constexpr int kScaleQ = QVEC ? BNQ : 4;
   __shared__ __align__(8) uint64_t bar_scale[kQMaxStages + 3];
@@ -247,11 +304,10 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
     abort_flag = 0;
     for (int s = 0; s < kQMaxStages; ++s) {
       mbar_init(smem_u32(&bar_full[s]), 1);
-      mbar_init(smem_u32(&bar_empty[s]), 1);
+      mbar_init(smem_u32(&bar_done[s]), 1);
     }
     for (int s = 0; s < kQMaxStages + 3; ++s) mbar_init(smem_u32(&bar_scale[s]), 32);
     for (int a = 0; a < 2; ++a) {
-      mbar_init(smem_u32(&bar_tmem_full[a]), 1);
       mbar_init(smem_u32(&bar_tmem_empty[a]), T::kDrainWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -275,15 +331,16 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
     int stage = 0, slot = 0, issued = 0;
     uint32_t phase = 0;
     bool ok = true;
-    const float* src_p[4];
+    uint32_t off_p[4];   // floats from the k-block's first scale
     constexpr int kPerQ = QVEC ? (BNQ + 31) / 32 : 1;
-    const float* src_q[kPerQ];
+    uint32_t off_q[kPerQ];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) src_p[i] = scale_at(p.sp, pt * 128 + lane + 32 * i) + (int64_t)kb0 * p.sp.s_k;
+    for (int i = 0; i < 4; ++i) off_p[i] = scale_offset(p.sp, pt * 128 + lane + 32 * i);
 #pragma unroll
-    for (int i = 0; i < kPerQ; ++i) src_q[i] = scale_at(p.sq, qt * BNQ + (QVEC ? lane + 32 * i : 0)) + (int64_t)kb0 * p.sq.s_k;
+    for (int i = 0; i < kPerQ; ++i) off_q[i] = scale_offset(p.sq, qt * BNQ + (QVEC ? lane + 32 * i : 0));
+    const float *src_p = p.sp.s + kb0 * p.sp.s_k, *src_q = p.sq.s + kb0 * p.sq.s_k;
     for (int kb = kb0; kb < kb1; ++kb) {
-      ok = __all_sync(0xffffffffu, q_wait(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag));
+      ok = __all_sync(0xffffffffu, q_wait(smem_u32(&bar_done[stage]), phase ^ 1u, &abort_flag));
       if (!ok) {
         if (lane == 0) report(p.status, 1, 1100 + stage, kb);
         break;
@@ -296,15 +353,12 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
         tma_load_2d(sp + kQStageP, &map_q, full, p.q_mn ? qt * BNQ : kb * 128, p.q_mn ? kb * 128 : qt * BNQ);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        copy_scale(smem_u32(&scale_p[slot][lane + 32 * i]), src_p[i]);
-        src_p[i] += p.sp.s_k;
-      }
+      for (int i = 0; i < 4; ++i) copy_scale(smem_u32(&scale_p[slot][lane + 32 * i]), src_p + off_p[i]);
 #pragma unroll
-      for (int i = 0; i < kPerQ; ++i) {
-        if (lane + 32 * i < kScaleQ) copy_scale(smem_u32(&scale_q[slot][lane + 32 * i]), src_q[i]);
-        src_q[i] += p.sq.s_k;
-      }
+      for (int i = 0; i < kPerQ; ++i)
+        if (lane + 32 * i < kScaleQ) copy_scale(smem_u32(&scale_q[slot][lane + 32 * i]), src_q + off_q[i]);
+      src_p += p.sp.s_k;
+      src_q += p.sq.s_k;
       arrive_after_copies(smem_u32(&bar_scale[slot]));
       ++issued;
       if (++slot == slots) slot = 0;
@@ -342,8 +396,7 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
           umma_e4m3(d, desc_p + at + kk * step_p, desc_q + at + kk * step_q, idesc, kk ? 1u : 0u);
-        tcgen05_commit(smem_u32(&bar_empty[stage]));
-        tcgen05_commit(smem_u32(&bar_tmem_full[acc]));
+        tcgen05_commit(smem_u32(&bar_done[stage]));
         if (++stage == p.stages) { stage = 0; phase ^= 1u; }
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
@@ -353,11 +406,11 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
     uint64_t sum[T::kCols / 2];
 #pragma unroll
     for (int j = 0; j < T::kCols / 2; ++j) sum[j] = 0;
-    int acc = 0, slot = 0;
-    uint32_t acc_phase = 0, slot_phase = 0;
+    int acc = 0, slot = 0, stage = 0;
+    uint32_t phase = 0, slot_phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
       bool ok = q_wait(smem_u32(&bar_scale[slot]), slot_phase, &abort_flag) &&
-                q_wait(smem_u32(&bar_tmem_full[acc]), acc_phase, &abort_flag);
+                q_wait(smem_u32(&bar_done[stage]), phase, &abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
         if (lane == 0) report(p.status, 4, 1400 + acc, kb);
@@ -365,12 +418,13 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
       }
       tcgen05_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BNQ + half * T::kCols);
-      drain_columns<T::kCols, QVEC>(sum, taddr, scale_p[slot][quarter * 32 + lane], &scale_q[slot][QVEC ? half * T::kCols : 0], [&] {
+      drain_columns<T::kCols, T::kCols < 32 ? T::kCols : 32, QVEC>(sum, taddr, scale_p[slot][quarter * 32 + lane], &scale_q[slot][QVEC ? half * T::kCols : 0], [&] {
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_tmem_empty[acc]));
       });
-      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      acc ^= 1;
+      if (++stage == p.stages) { stage = 0; phase ^= 1u; }
       if (++slot == slots) { slot = 0; slot_phase ^= 1u; }
     }
     // Every load has landed and every MMA has read it: the ring is free for the partial sums.
@@ -417,20 +471,40 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
   }
 }
 
-// ---- large products: CTA pairs ---------------------------------------------------------------------------------------
+// ---- large products with power-of-two scales: CTA pairs, scales applied by the tensor pipe ---------------------------------
 // The two CTAs of a cluster share a 256 x 256 tile (tcgen05 cta_group::2): each stages 128 rows of P and 128 of Q per
-// k-block (32 KiB a stage, five stages), the MMA of CTA 0 reads Q from both, each CTA drains the sums of its own 128 rows.
-// Persistent over the tiles; barriers as in gemm_tc_pair.cu.  At the tensor pipe's rate a k-block takes 512 clocks, in
-// which the eight drain warps read 128 x 256 sums from TMEM and add them, scaled, to 128 running sums a thread.
-constexpr int kQPairStages = 5;
-constexpr int kQPairSlots = kQPairStages + 3;
+// k-block (32 KiB a stage), the MMA issued by CTA 0 reads Q from both, each CTA drains the sums of its own 128 rows.
+//
+// tcgen05.mma.kind::mxf8f6f4.block_scale multiplies every 32 products by a power of two per row of P and one per row of Q,
+// given as exponent bytes in TMEM.  A scale that is a power of two is its f32 exponent field, so two warps fetch the
+// scales, keep bits 23-30 of each, and pack four k-blocks' bytes of an element into one word (the instruction descriptor
+// selects the byte); the issuer copies the words to TMEM once per four k-blocks.  The partial sums then need no work per k-block:
+// the accumulator runs over eight (1024 terms) before the drain warps add it to 64 running sums a thread with
+// round-to-nearest, which bounds what the tensor pipe's truncating adds can lose (32 adds of at most 2^-23).
+//
+// Layout of the words, in shared memory and TMEM: element r of 128 at row r % 32, word r / 32 of a row of four; TMEM holds it
+// in four columns of 32 lanes, repeated in all four lane quarters (tcgen05.cp ... 32x128b.warpx4).  P: the CTA's own 128 rows;
+// Q: all 256, in both CTAs.
+//
+// Measured against the drain that scales every k-block itself (as gemm_q_kernel does), same tile: 8192^3 577 us (one scale for
+// 128 columns) and 1030 us (one per column), the pipe waiting for the drain's multiplies.
+constexpr int kQPairDrainWarps = 16;
+constexpr int kQPairCols = 64;                               // columns a drain warp sums: a quarter of the tile
+constexpr int kQPairThreads = 128 + 32 * kQPairDrainWarps;   // warp 0 TMA, 1 MMA, 2 scales of P, 3 scales of Q
+constexpr int kQPairStages = 4;                              // k-block kb of a tile is in stage kb % 4
 constexpr int kQPairStageBytes = 2 * kQStageP;
 constexpr int kQPairRing = kQPairStages * kQPairStageBytes;
-constexpr int kQPairSmem = kQPairRing + kEpiWarps * 32 * 128 + 1024;
+constexpr int kQPairStaging = 32 * 128;                      // bytes of a drain warp's staging tile: 32 rows x 32 columns
+constexpr int kQPairSmem = kQPairRing + kQPairDrainWarps * kQPairStaging + 1024;
+constexpr int kQGroup = 4;                                   // k-blocks whose scales share a word: one turn of the ring
+constexpr int kQChunk = 8;                                   // k-blocks summed in TMEM
+constexpr int kQAhead = 8;                                   // k-blocks between the L2 prefetch of a box and its load
+constexpr int kQScaleSlots = 4;
+constexpr int kQScaleSlotBytes = 3 * 512;                    // [P | Q 0..127 | Q 128..255]
+constexpr int kQScaleCol = 256;                              // TMEM columns behind the accumulator: two sets of 4 + 8
 
 struct QPairParams {
-  TcParams t;             // c, bias, act, m, n, num_kb, mblks, nblks, pair_group_m, c_tma, status
-  int p_mn, q_mn;
+  TcParams t;             // c, bias, act, m, n, num_kb, mblks, nblks, pair_group_m, status
   QScales sp, sq;
 };
 
@@ -440,21 +514,36 @@ __device__ __forceinline__ void tma_pair_load_2d(uint32_t dst, const CUtensorMap
       ::"r"(dst), "l"(map), "r"(bar_cluster), "r"(c0), "r"(c1)
       : "memory");
 }
-__device__ __forceinline__ void umma_e4m3_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                               uint32_t accumulate) {
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1) : "memory");
+}
+// D[tmem] (+)= (A[smem] * scale) (B[smem] * scale), e4m3 inputs, one exponent byte per 32 along k, f32 accumulate, K = 32.
+__device__ __forceinline__ void umma_e4m3_scaled_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                      uint32_t a_scale_tmem, uint32_t b_scale_tmem, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scale_tmem), "r"(b_scale_tmem), "r"(accumulate)
       : "memory");
+}
+// Both operands e4m3 (format 0), scales as exponent bytes (bit 23), bits 15 / 16: MN-major A / B, N >> 3, M >> 4.  The byte of a
+// scale word: bits 29-30 for A, 4-5 for B.
+__host__ __device__ constexpr uint32_t instr_desc_e4m3_scaled(int a_mn, int b_mn, int m, int n) {
+  return (1u << 23) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t scale_byte_select(int i) { return ((uint32_t)i << 29) | ((uint32_t)i << 4); }
+// 32 rows of 16 bytes of shared memory (unswizzled, 8-row groups 128 bytes apart) to 4 columns of TMEM, in both CTAs.
+__device__ __forceinline__ void copy_scales_pair(uint32_t tmem, uint32_t smem) {
+  const uint64_t desc = make_smem_desc(smem, 128u, 0u, 0u);
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
 // Adds the bias, applies the activation and stores a drain warp's 32 x 32 block of C whose first element is (row0, col0);
 // lane r holds row r.  The block passes through the warp's staging tile (16-byte word j of row r at slot j ^ (r & 7):
-// conflict free, and TMA's 128-byte swizzle) and leaves as one bulk tensor store, which clips what lies outside C, or, where
-// no tensor map describes C, as 128-byte rows.
-__device__ __forceinline__ void store_q_block(float (&v)[32], const TcParams& p, const CUtensorMap* map_c, float4* stage,
-                                              int row0, int col0, int lane) {
+// conflict free both ways), so that every store instruction writes whole 128-byte lines.  Plain stores: bulk tensor stores of the
+// same tile queue in the copy engine before the next tile's loads, which then took 3000 to 4700 clocks to arrive.
+__device__ __forceinline__ void store_q_block(float (&v)[32], const TcParams& p, float4* stage, int row0, int col0, int lane,
+                                              bool vec_ok) {
   if (row0 >= p.m || col0 >= p.n) return;   // uniform over the warp
   if (p.bias != nullptr) {
     if (col0 + 32 <= p.n && (reinterpret_cast<uintptr_t>(p.bias + col0) & 15u) == 0) {
@@ -482,33 +571,28 @@ __device__ __forceinline__ void store_q_block(float (&v)[32], const TcParams& p,
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = q_epilogue(v[j], CLEAVE_ACT_RELU);
   }
-  if (p.c_tma) {
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the tile's last store has been read
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      stage[lane * 8 + (j ^ (lane & 7))] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // generic writes -> visible to the copy engine
-    __syncwarp();
-    if (lane == 0) {
-      asm volatile(
-          "cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
-          ::"l"(map_c), "r"(smem_u32(stage)), "r"(col0), "r"(row0), "r"(0)
-          : "memory");
-      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-    }
-    return;
-  }
-  __syncwarp();
+  __syncwarp();   // the tile's last block has been read
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     stage[lane * 8 + (j ^ (lane & 7))] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
   __syncwarp();
+  if (vec_ok) {   // C is 16-byte aligned and n a multiple of 4
+    const int slot = lane & 7;
+    if (col0 + 4 * slot < p.n) {
+      float* dst = p.c + (int64_t)row0 * p.n + col0 + 4 * slot;
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const int r = it * 4 + (lane >> 3);
+        if (row0 + r < p.m) *reinterpret_cast<float4*>(dst + (int64_t)r * p.n) = stage[r * 8 + (slot ^ (r & 7))];
+      }
+    }
+    return;
+  }
   const float* words = reinterpret_cast<const float*>(stage);
-  const int rows = p.m - row0 < 32 ? p.m - row0 : 32;
   if (col0 + lane < p.n) {
     float* dst = p.c + (int64_t)row0 * p.n + col0 + lane;
-    for (int r = 0; r < rows; ++r) dst[(int64_t)r * p.n] = words[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)];
+    for (int r = 0; r < 32 && row0 + r < p.m; ++r)
+      dst[(int64_t)r * p.n] = words[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)];
   }
 }
 
@@ -521,19 +605,19 @@ __device__ __forceinline__ void decode_q_tile(int t, const TcParams& p, int& mb,
   nb = r / rows_here;
 }
 
-template <bool QVEC>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+template <int P_MN, int Q_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kQPairThreads, 1)
 gemm_q_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
-                   const __grid_constant__ CUtensorMap map_c, const QPairParams p) {
+                   const QPairParams p) {
   extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(128) uint8_t scale_words[kQScaleSlots][kQScaleSlotBytes];
+  // full / done: a stage's bytes have landed (in CTA 0, for both) / its MMAs have read them; scale_full / scale_empty: the
+  // same for a slot of scale words; acc_full / acc_empty: the accumulator is complete / has been read (in CTA 0)
   __shared__ __align__(8) uint64_t bar_full[kQPairStages];
-  __shared__ __align__(8) uint64_t bar_empty[kQPairStages];
-  __shared__ __align__(8) uint64_t bar_tmem_full[kAccStages];
-  __shared__ __align__(8) uint64_t bar_tmem_empty[kAccStages];
-  constexpr int kScaleQ = QVEC ? 256 : 4;   // one value for each 128 columns, or one for every column
-  __shared__ __align__(8) uint64_t bar_scale[kQPairSlots];
-  __shared__ __align__(16) float scale_p[kQPairSlots][128];
-  __shared__ __align__(16) float scale_q[kQPairSlots][kScaleQ];
+  __shared__ __align__(8) uint64_t bar_done[kQPairStages];
+  __shared__ __align__(8) uint64_t bar_scale_full[kQScaleSlots];
+  __shared__ __align__(8) uint64_t bar_scale_empty[kQScaleSlots];
+  __shared__ __align__(8) uint64_t bar_acc_full, bar_acc_empty;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
 
@@ -546,13 +630,14 @@ gemm_q_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
     abort_flag = 0;
     for (int s = 0; s < kQPairStages; ++s) {
       mbar_init(smem_u32(&bar_full[s]), 1);
-      mbar_init(smem_u32(&bar_empty[s]), 1);
+      mbar_init(smem_u32(&bar_done[s]), 1);
     }
-    for (int s = 0; s < kQPairSlots; ++s) mbar_init(smem_u32(&bar_scale[s]), 32);
-    for (int a = 0; a < kAccStages; ++a) {
-      mbar_init(smem_u32(&bar_tmem_full[a]), 1);
-      mbar_init(smem_u32(&bar_tmem_empty[a]), 2 * kEpiWarps);   // the drain warps of both CTAs
+    for (int s = 0; s < kQScaleSlots; ++s) {
+      mbar_init(smem_u32(&bar_scale_full[s]), 4);   // two scale warps in each CTA
+      mbar_init(smem_u32(&bar_scale_empty[s]), 1);
     }
+    mbar_init(smem_u32(&bar_acc_full), 1);
+    mbar_init(smem_u32(&bar_acc_empty), 2 * kQPairDrainWarps);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -569,141 +654,222 @@ gemm_q_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
   const uint32_t tmem_base = tmem_slot;
 
   if (warp == 0) {
-    if (lane == 0) {
+    // ---- bytes
+    if (elect_one()) {
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_p) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
     }
-    int stage = 0, slot = 0, issued = 0;
-    uint32_t phase = 0;
+    uint32_t phases = 0, used = 0;   // a bit a stage: the parity of its next fill; filled at all
     bool ok = true;
     for (int t = blockIdx.x >> 1; ok && t < tiles; t += n_clusters) {
       int mb, nb;
       decode_q_tile(t, p.t, mb, nb);
       const int p0 = mb * 256 + (int)rank * 128, q0 = nb * 256 + (int)rank * 128;
-      const float* src_p[4];
-      constexpr int kPerQ = QVEC ? 8 : 1;
-      const float* src_q[kPerQ];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) src_p[i] = scale_at(p.sp, p0 + lane + 32 * i);
-#pragma unroll
-      for (int i = 0; i < kPerQ; ++i) src_q[i] = scale_at(p.sq, nb * 256 + (QVEC ? lane + 32 * i : (lane & 1) * 128));
       for (int kb = 0; kb < num_kb; ++kb) {
-        ok = __all_sync(0xffffffffu, q_wait(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag));
+        const int stage = kb % kQPairStages;
+        ok = __all_sync(0xffffffffu, q_wait(smem_u32(&bar_done[stage]), ((phases >> stage) & 1u) ^ 1u, &abort_flag));
         if (!ok) {
           if (lane == 0) report(p.t.status, 1, 1500 + stage, kb);
           break;
         }
-        if (lane == 0) {
+        if (elect_one()) {
+          // The pairs at work share panels -- a panel of P is read by those of one mb, of Q by those of one nb -- and walk k
+          // together, so every k-block comes from HBM once, some 3400 clocks behind the request: more than the ring covers.
+          // The pairs of a panel take turns to fetch it into L2 ahead of time.
+          int ahead = kb + kQAhead, pf_p = p0, pf_q = q0, pf_mb = mb, pf_nb = nb;
+          bool fetch = true;
+          if (ahead >= num_kb) {
+            ahead -= num_kb;
+            fetch = t + n_clusters < tiles && ahead < num_kb;
+            if (fetch) {
+              decode_q_tile(t + n_clusters, p.t, pf_mb, pf_nb);
+              pf_p = pf_mb * 256 + (int)rank * 128;
+              pf_q = pf_nb * 256 + (int)rank * 128;
+            }
+          }
+          if (fetch && (pf_nb + ahead) % 8 == 0) tma_prefetch_2d(&map_p, P_MN ? pf_p : ahead * 128, P_MN ? ahead * 128 : pf_p);
+          if (fetch && (pf_mb + ahead) % 8 == 0) tma_prefetch_2d(&map_q, Q_MN ? pf_q : ahead * 128, Q_MN ? ahead * 128 : pf_q);
           const uint32_t full_own = smem_u32(&bar_full[stage]);
           const uint32_t full0 = map_to_cta(full_own, 0);
           if (rank == 0) mbar_arrive_expect_tx(full_own, 2 * kQPairStageBytes);   // both CTAs' boxes
           const uint32_t sp = ring + stage * kQPairStageBytes;
-          tma_pair_load_2d(sp, &map_p, full0, p.p_mn ? p0 : kb * 128, p.p_mn ? kb * 128 : p0);
-          tma_pair_load_2d(sp + kQStageP, &map_q, full0, p.q_mn ? q0 : kb * 128, p.q_mn ? kb * 128 : q0);
+          tma_pair_load_2d(sp, &map_p, full0, P_MN ? p0 : kb * 128, P_MN ? kb * 128 : p0);
+          tma_pair_load_2d(sp + kQStageP, &map_q, full0, Q_MN ? q0 : kb * 128, Q_MN ? kb * 128 : q0);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          copy_scale(smem_u32(&scale_p[slot][lane + 32 * i]), src_p[i]);
-          src_p[i] += p.sp.s_k;
-        }
-#pragma unroll
-        for (int i = 0; i < kPerQ; ++i) {
-          if (lane + 32 * i < kScaleQ) copy_scale(smem_u32(&scale_q[slot][lane + 32 * i]), src_q[i]);
-          src_q[i] += p.sq.s_k;
-        }
-        arrive_after_copies(smem_u32(&bar_scale[slot]));
-        ++issued;
-        if (++slot == kQPairSlots) slot = 0;
-        if (++stage == kQPairStages) { stage = 0; phase ^= 1u; }
+        __syncwarp();
+        phases ^= 1u << stage;
+        used |= 1u << stage;
       }
     }
-    if (!ok) {
+    if (!ok && rank == 0 && lane == 0) {
       // leaving early: give the copies in flight a bounded chance to land (CTA 0 sees their completion)
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      for (int s = 0; rank == 0 && lane == 0 && s < kQPairStages; ++s) {
-        const int fills = (issued + kQPairStages - 1 - s) / kQPairStages;
-        if (fills == 0) continue;
-        for (int spin = 0; spin < (1 << 20); ++spin)
-          if (mbar_try_wait(smem_u32(&bar_full[s]), (uint32_t)(fills - 1) & 1u)) break;
-      }
+      for (int s = 0; s < kQPairStages; ++s)
+        for (int spin = 0; ((used >> s) & 1u) && spin < (1 << 20); ++spin)
+          if (mbar_try_wait(smem_u32(&bar_full[s]), ((phases >> s) & 1u) ^ 1u)) break;
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      const uint32_t idesc = instr_desc_e4m3(p.p_mn, p.q_mn, 256, 256);
-      const uint64_t desc_p = operand_desc(ring, p.p_mn, 0), desc_q = operand_desc(ring + kQStageP, p.q_mn, 0);
-      const uint64_t step_p = k_step(p.p_mn), step_q = k_step(p.q_mn);
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
+    // ---- MMAs, CTA 0 for both.  The whole warp runs the loop, so that its state stays in uniform registers; one lane issues.
+    if (rank == 0) {
+      constexpr uint32_t idesc = instr_desc_e4m3_scaled(P_MN, Q_MN, 256, 256);
+      const uint64_t desc_p = operand_desc(ring, P_MN, 0), desc_q = operand_desc(ring + kQStageP, Q_MN, 0);
+      const int my_tiles = (tiles - (int)(blockIdx.x >> 1) + n_clusters - 1) / n_clusters;
+      const int groups = my_tiles * ((num_kb + kQGroup - 1) / kQGroup);
+      uint32_t phases = 0, acc_phase = 0;
       bool ok = true;
+      // The scale words of group g (counted over the tiles) go to TMEM while the group before it is being multiplied.
+      auto fetch_scales = [&](int g) {
+        const int slot = g % kQScaleSlots;
+        ok = __all_sync(0xffffffffu, q_wait<true>(smem_u32(&bar_scale_full[slot]), (uint32_t)(g / kQScaleSlots) & 1u, &abort_flag));
+        if (!ok) {
+          if (lane == 0) report(p.t.status, 2, 1600 + slot, g);
+          return;
+        }
+        tcgen05_fence_after();
+        if (elect_one()) {   // ordered before the MMAs that follow from this thread
+          const uint32_t scales = tmem_base + kQScaleCol + (uint32_t)(g & 1) * 16u;
+          const uint32_t words = smem_u32(&scale_words[slot][0]);
+          copy_scales_pair(scales, words);
+          copy_scales_pair(scales + 4, words + 512);
+          copy_scales_pair(scales + 8, words + 1024);
+        }
+        __syncwarp();
+      };
+      int g = 0;
+      fetch_scales(0);
       for (int t = blockIdx.x >> 1; ok && t < tiles; t += n_clusters) {
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!q_wait(smem_u32(&bar_tmem_empty[acc]), acc_phase ^ 1u, &abort_flag)) {
-            report(p.t.status, 2, 1600 + acc, kb);
-            ok = false;
-            break;
+        for (int kb0 = 0; ok && kb0 < num_kb; kb0 += kQGroup, ++g) {
+          const bool chunk_start = kb0 % kQChunk == 0;
+          if (chunk_start) {
+            ok = __all_sync(0xffffffffu, q_wait(smem_u32(&bar_acc_empty), acc_phase ^ 1u, &abort_flag));
+            if (!ok) {
+              if (lane == 0) report(p.t.status, 5, 1650, kb0);
+              break;
+            }
           }
-          if (!q_wait(smem_u32(&bar_full[stage]), phase, &abort_flag)) {
-            report(p.t.status, 3, 1700 + stage, kb);
-            ok = false;
-            break;
-          }
-          tcgen05_fence_after();
-          const uint64_t at = (uint64_t)(stage * kQPairStageBytes) >> 4;
-          const uint32_t d = tmem_base + (uint32_t)(acc * BN);
+          const uint32_t scales = tmem_base + kQScaleCol + (uint32_t)(g & 1) * 16u;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_e4m3_pair(d, desc_p + at + kk * step_p, desc_q + at + kk * step_q, idesc, kk ? 1u : 0u);
-          tcgen05_commit_pair(smem_u32(&bar_empty[stage]));
-          tcgen05_commit_pair(smem_u32(&bar_tmem_full[acc]));
-          if (++stage == kQPairStages) { stage = 0; phase ^= 1u; }
-          if (++acc == kAccStages) { acc = 0; acc_phase ^= 1u; }
+          for (int s = 0; s < kQGroup; ++s) {
+            if (kb0 + s >= num_kb) break;
+            ok = __all_sync(0xffffffffu, q_wait(smem_u32(&bar_full[s]), (phases >> s) & 1u, &abort_flag));
+            if (!ok) {
+              if (lane == 0) report(p.t.status, 3, 1700 + s, kb0);
+              break;
+            }
+            tcgen05_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                umma_e4m3_scaled_pair(tmem_base, desc_p + (uint32_t)((s * kQPairStageBytes + kk * (P_MN ? 4096 : 32)) >> 4),
+                                      desc_q + (uint32_t)((s * kQPairStageBytes + kk * (Q_MN ? 4096 : 32)) >> 4),
+                                      idesc | scale_byte_select(s), scales, scales + 4,
+                                      s == 0 && kk == 0 && chunk_start ? 0u : 1u);
+              tcgen05_commit_pair(smem_u32(&bar_done[s]));
+            }
+            __syncwarp();
+            phases ^= 1u << s;
+          }
+          if (!ok) break;
+          const bool chunk_end = kb0 + kQGroup >= num_kb || kb0 % kQChunk != 0;
+          if (elect_one()) {
+            if (chunk_end) tcgen05_commit_pair(smem_u32(&bar_acc_full));
+            tcgen05_commit_pair(smem_u32(&bar_scale_empty[g % kQScaleSlots]));
+          }
+          __syncwarp();
+          if (chunk_end) acc_phase ^= 1u;
+          if (g + 1 < groups) fetch_scales(g + 1);
         }
       }
     }
-  } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    int acc = 0, slot = 0;
-    uint32_t acc_phase = 0, slot_phase = 0;
-    float4* stage_tile = reinterpret_cast<float4*>(smem_raw + (ring - smem_u32(smem_raw)) + kQPairRing) + (warp - 2) * (32 * 8);
+  } else if (warp < 4) {
+    // ---- scales: warp 2 the CTA's 128 rows of P, warp 3 the tile's 256 of Q
+    const bool for_q = warp == 3;
+    const QScales& o = for_q ? p.sq : p.sp;
+    int slot = 0;
+    uint32_t slot_phase = 0;
     bool ok = true;
     for (int t = blockIdx.x >> 1; ok && t < tiles; t += n_clusters) {
       int mb, nb;
       decode_q_tile(t, p.t, mb, nb);
-      uint64_t sum[64];
+      const int first = for_q ? nb * 256 : mb * 256 + (int)rank * 128;
+      for (int kb0 = 0; kb0 < num_kb; kb0 += kQGroup) {
+        uint32_t w[2][4];
 #pragma unroll
-      for (int j = 0; j < 64; ++j) sum[j] = 0;
-      for (int kb = 0; kb < num_kb; ++kb) {
-        ok = q_wait(smem_u32(&bar_scale[slot]), slot_phase, &abort_flag) &&
-             q_wait(smem_u32(&bar_tmem_full[acc]), acc_phase, &abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1 && !for_q) break;
+          uint32_t bits[4][kQGroup];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float* src = o.s + scale_offset(o, first + h * 128 + i * 32 + lane) + (int64_t)kb0 * o.s_k;
+#pragma unroll
+            for (int j = 0; j < kQGroup; ++j)
+              bits[i][j] = kb0 + j < num_kb ? __float_as_uint(__ldg(src + j * o.s_k)) : 0u;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[h][i] = ((bits[i][0] >> 23) & 0xffu) | (((bits[i][1] >> 23) & 0xffu) << 8) | (((bits[i][2] >> 23) & 0xffu) << 16) |
+                      (((bits[i][3] >> 23) & 0xffu) << 24);
+        }
+        ok = __all_sync(0xffffffffu, q_wait(smem_u32(&bar_scale_empty[slot]), slot_phase ^ 1u, &abort_flag));
         if (!ok) {
-          if (lane == 0) report(p.t.status, 4, 1800 + acc, kb);
+          if (lane == 0) report(p.t.status, 3, 1700 + slot, kb0);
+          break;
+        }
+        uint4* dst = reinterpret_cast<uint4*>(&scale_words[slot][for_q ? 512 : 0]) + lane;
+        dst[0] = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
+        if (for_q) dst[32] = make_uint4(w[1][0], w[1][1], w[1][2], w[1][3]);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // generic writes -> visible to the copy to TMEM
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_scale_full[slot]), 0));
+        if (++slot == kQScaleSlots) { slot = 0; slot_phase ^= 1u; }
+      }
+    }
+  } else {
+    // ---- drain and epilogue
+    const int quarter = warp & 3, part = (warp - 4) >> 2;   // TMEM lanes 32 * quarter .., columns 64 * part ..
+    uint32_t acc_phase = 0;
+    float4* stage_tile = reinterpret_cast<float4*>(smem_raw + (ring - smem_u32(smem_raw)) + kQPairRing + (warp - 4) * kQPairStaging);
+    const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(part * kQPairCols);
+    const bool vec_ok = p.t.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.t.c) & 15u) == 0;
+    const uint32_t acc_empty0 = map_to_cta(smem_u32(&bar_acc_empty), 0);
+    bool ok = true;
+    for (int t = blockIdx.x >> 1; ok && t < tiles; t += n_clusters) {
+      int mb, nb;
+      decode_q_tile(t, p.t, mb, nb);
+      float sum[kQPairCols];
+#pragma unroll
+      for (int j = 0; j < kQPairCols; ++j) sum[j] = 0.0f;
+      for (int kb = 0; kb < num_kb; kb += kQChunk) {
+        ok = __all_sync(0xffffffffu, q_wait(smem_u32(&bar_acc_full), acc_phase, &abort_flag));
+        if (!ok) {
+          if (lane == 0) report(p.t.status, 4, 1800, kb);
           break;
         }
         tcgen05_fence_after();
-        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN + half * 128);
-        drain_columns<128, QVEC>(sum, taddr, scale_p[slot][quarter * 32 + lane], &scale_q[slot][QVEC ? half * 128 : half], [&] {
-          tcgen05_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&bar_tmem_empty[acc]), 0));
-        });
-        if (++acc == kAccStages) { acc = 0; acc_phase ^= 1u; }
-        if (++slot == kQPairSlots) { slot = 0; slot_phase ^= 1u; }
+#pragma unroll
+        for (int g = 0; g < kQPairCols / 16; ++g) {
+          uint32_t r[16];
+          tmem_ld_16(taddr + g * 16, r);
+          tmem_wait_16(r);
+          if (g == kQPairCols / 16 - 1) {   // all columns are in registers: the accumulator is free
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty0);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sum[g * 16 + j] = __fadd_rn(sum[g * 16 + j], __uint_as_float(r[j]));
+        }
+        acc_phase ^= 1u;
       }
       if (!ok) break;
 #pragma unroll
-      for (int pass = 0; pass < 4; ++pass) {
+      for (int pass = 0; pass < kQPairCols / 32; ++pass) {
         float v[32];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          v[2 * j] = low_half(sum[pass * 16 + j]);
-          v[2 * j + 1] = high_half(sum[pass * 16 + j]);
-        }
-        store_q_block(v, p.t, &map_c, stage_tile, mb * 256 + (int)rank * 128 + quarter * 32, nb * 256 + half * 128 + 32 * pass,
-                      lane);
+        for (int j = 0; j < 32; ++j) v[j] = sum[pass * 32 + j];
+        store_q_block(v, p.t, stage_tile, mb * 256 + (int)rank * 128 + quarter * 32, nb * 256 + part * kQPairCols + 32 * pass, lane,
+                      vec_ok);
       }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // stores have reached memory
   }
 
   __syncwarp();
@@ -784,19 +950,19 @@ static bool launch_q(const CUtensorMap& map_p, const CUtensorMap& map_q, const Q
   return ok;
 }
 
-template <bool QVEC>
+template <int P_MN, int Q_MN>
 static bool launch_q_pair(const CUtensorMap* maps, const QPairParams& p) {
   static bool attr_set = false;
   if (!attr_set) {
-    if (!cuda_ok(cudaFuncSetAttribute(gemm_q_pair_kernel<QVEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, kQPairSmem),
+    if (!cuda_ok(cudaFuncSetAttribute(gemm_q_pair_kernel<P_MN, Q_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kQPairSmem),
                  "cudaFuncSetAttribute(8-bit pair gemm)"))
       return false;
     attr_set = true;
   }
   const int tiles = p.t.mblks * p.t.nblks, pairs = ctx().sm_count / 2;
   profile_mark(true);
-  gemm_q_pair_kernel<QVEC><<<2 * (tiles < pairs ? tiles : pairs), kGemmThreads, kQPairSmem, ctx().stream>>>(maps[0], maps[1],
-                                                                                                         maps[2], p);
+  gemm_q_pair_kernel<P_MN, Q_MN><<<2 * (tiles < pairs ? tiles : pairs), kQPairThreads, kQPairSmem, ctx().stream>>>(
+      maps[0], maps[1], p);
   count_launch();
   const bool ok = cuda_ok(cudaGetLastError(), "8-bit pair GEMM launch");
   profile_mark(false);
@@ -815,16 +981,12 @@ static bool gemm_q_pairs(const QSide& a, const QSide& b, float* c, const float* 
   p.t.nblks = ceil_div(b.dim, 256);
   p.t.pair_group_m = 8;
   p.t.status = ctx().status_dev;
-  p.p_mn = a.mn;
-  p.q_mn = b.mn;
   p.sp = side_scales(a);
   p.sq = side_scales(b);
-  CUtensorMap maps[3];
+  CUtensorMap maps[2];
   if (!side_map(&maps[0], a, 128) || !side_map(&maps[1], b, 128)) return false;
-  maps[2] = maps[0];
-  // whole 32 x 32 blocks of C leave as bulk tensor stores where a tensor map can describe C
-  p.t.c_tma = aligned16(c) && b.dim % 4 == 0 && make_c_map(&maps[2], c, a.dim, b.dim, 1, 1) ? 1 : 0;
-  return b.blocks == CLEAVE_BLOCKS_TILES ? launch_q_pair<false>(maps, p) : launch_q_pair<true>(maps, p);
+  return a.mn ? (b.mn ? launch_q_pair<1, 1>(maps, p) : launch_q_pair<1, 0>(maps, p))
+              : (b.mn ? launch_q_pair<0, 1>(maps, p) : launch_q_pair<0, 0>(maps, p));
 }
 
 static bool gemm_q(const QSide& a, const QSide& b, float* c, const float* bias, int act) {

@@ -1050,7 +1050,7 @@ static bool launch_split_k(const GemmArgs& g, int slices) {
   return ok;
 }
 
-bool make_c_map(CUtensorMap* map, float* c, int m, int n, int batch, int mode);
+static bool make_c_map(CUtensorMap* map, float* c, int m, int n, int batch, int mode);
 
 // hi planes are the caller's tensors, lo planes come from one streaming pass per operand.
 static bool launch_lo_plane(const GemmArgs& g) {
@@ -1170,7 +1170,7 @@ static bool launch_lo_plane(const GemmArgs& g) {
 // Tensor map over the output for TMA stores: dims {n, m, batch}; box 32 x 32 floats with the 128-byte swizzle
 // (mode 1: the layout of a drain warp's shared staging tile) or 16 columns x 32 rows with the 64-byte swizzle
 // (mode 2: the layout of its halves).  Needs a 16-byte aligned C and n a multiple of 4.
-bool make_c_map(CUtensorMap* map, float* c, int m, int n, int batch, int mode) {
+static bool make_c_map(CUtensorMap* map, float* c, int m, int n, int batch, int mode) {
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) return false;
   cuuint64_t dims[3] = {(cuuint64_t)n, (cuuint64_t)m, (cuuint64_t)batch};
