@@ -2,9 +2,10 @@
 //
 //   C[m, n] = act( sum over k-blocks kb of  sA(m, kb) * sB(n, kb) * sum over k in kb of qA(m, k) * qB(n, k)  + bias[n] )
 //
-// tcgen05.mma.kind::f8f6f4 multiplies the e4m3 bytes and adds up one 128-wide k-block in TMEM (four instructions of K = 32);
-// the drain warps read that partial sum, multiply it by the two scales and add it to running sums in registers with
-// round-to-nearest.  So scales may be any f32 values, and the tensor pipe's truncating adds never run over more than 128 terms.
+// Two kernels.  gemm_q_kernel: tcgen05.mma.kind::f8f6f4 multiplies the e4m3 bytes and adds up one 128-wide k-block in TMEM
+// (four instructions of K = 32); the drain warps read that partial sum, multiply it by the two scales and add it to running sums
+// in registers with round-to-nearest.  So scales may be any f32 values.  gemm_q_pair_kernel, for large products whose scales
+// are powers of two (the quantizer's are): the tensor pipe applies the scales itself.
 //
 // Operands are read where they lie, in either order: stored with k contiguous (K-major) or with the row / column index
 // contiguous (MN-major); 8-bit operands take the 128-byte swizzle both ways, a 128 x 128 box is 16 KiB.  Out-of-range
@@ -498,7 +499,6 @@ constexpr int kQPairStaging = 32 * 128;                      // bytes of a drain
 constexpr int kQPairSmem = kQPairRing + kQPairDrainWarps * kQPairStaging + 1024;
 constexpr int kQGroup = 4;                                   // k-blocks whose scales share a word: one turn of the ring
 constexpr int kQChunk = 8;                                   // k-blocks summed in TMEM
-constexpr int kQAhead = 8;                                   // k-blocks between the L2 prefetch of a box and its load
 constexpr int kQScaleSlots = 4;
 constexpr int kQScaleSlotBytes = 3 * 512;                    // [P | Q 0..127 | Q 128..255]
 constexpr int kQScaleCol = 256;                              // TMEM columns behind the accumulator: two sets of 4 + 8
@@ -513,9 +513,6 @@ __device__ __forceinline__ void tma_pair_load_2d(uint32_t dst, const CUtensorMap
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
       ::"r"(dst), "l"(map), "r"(bar_cluster), "r"(c0), "r"(c1)
       : "memory");
-}
-__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int c0, int c1) {
-  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1) : "memory");
 }
 // D[tmem] (+)= (A[smem] * scale) (B[smem] * scale), e4m3 inputs, one exponent byte per 32 along k, f32 accumulate, K = 32.
 __device__ __forceinline__ void umma_e4m3_scaled_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
@@ -633,7 +630,7 @@ gemm_q_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
       mbar_init(smem_u32(&bar_done[s]), 1);
     }
     for (int s = 0; s < kQScaleSlots; ++s) {
-      mbar_init(smem_u32(&bar_scale_full[s]), 4);   // two scale warps in each CTA
+      mbar_init(smem_u32(&bar_scale_full[s]), rank == 0 ? 3 : 2);   // the CTA's two scale warps; in CTA 0 also CTA 1's word for its own
       mbar_init(smem_u32(&bar_scale_empty[s]), 1);
     }
     mbar_init(smem_u32(&bar_acc_full), 1);
@@ -673,22 +670,6 @@ gemm_q_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
           break;
         }
         if (elect_one()) {
-          // The pairs at work share panels -- a panel of P is read by those of one mb, of Q by those of one nb -- and walk k
-          // together, so every k-block comes from HBM once, some 3400 clocks behind the request: more than the ring covers.
-          // The pairs of a panel take turns to fetch it into L2 ahead of time.
-          int ahead = kb + kQAhead, pf_p = p0, pf_q = q0, pf_mb = mb, pf_nb = nb;
-          bool fetch = true;
-          if (ahead >= num_kb) {
-            ahead -= num_kb;
-            fetch = t + n_clusters < tiles && ahead < num_kb;
-            if (fetch) {
-              decode_q_tile(t + n_clusters, p.t, pf_mb, pf_nb);
-              pf_p = pf_mb * 256 + (int)rank * 128;
-              pf_q = pf_nb * 256 + (int)rank * 128;
-            }
-          }
-          if (fetch && (pf_nb + ahead) % 8 == 0) tma_prefetch_2d(&map_p, P_MN ? pf_p : ahead * 128, P_MN ? ahead * 128 : pf_p);
-          if (fetch && (pf_mb + ahead) % 8 == 0) tma_prefetch_2d(&map_q, Q_MN ? pf_q : ahead * 128, Q_MN ? ahead * 128 : pf_q);
           const uint32_t full_own = smem_u32(&bar_full[stage]);
           const uint32_t full0 = map_to_cta(full_own, 0);
           if (rank == 0) mbar_arrive_expect_tx(full_own, 2 * kQPairStageBytes);   // both CTAs' boxes
@@ -769,7 +750,7 @@ gemm_q_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
             phases ^= 1u << s;
           }
           if (!ok) break;
-          const bool chunk_end = kb0 + kQGroup >= num_kb || kb0 % kQChunk != 0;
+          const bool chunk_end = kb0 + kQGroup >= num_kb || kb0 % kQChunk == kQChunk - kQGroup;
           if (elect_one()) {
             if (chunk_end) tcgen05_commit_pair(smem_u32(&bar_acc_full));
             tcgen05_commit_pair(smem_u32(&bar_scale_empty[g % kQScaleSlots]));
@@ -778,6 +759,21 @@ gemm_q_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
           if (chunk_end) acc_phase ^= 1u;
           if (g + 1 < groups) fetch_scales(g + 1);
         }
+      }
+    }
+    else {
+      // CTA 1 tells CTA 0 that its scale words are there.  The release that another CTA's copy to TMEM needs takes a thousand
+      // clocks; here they delay nobody.
+      const int my_tiles = (tiles - (int)(blockIdx.x >> 1) + n_clusters - 1) / n_clusters;
+      const int groups = my_tiles * ((num_kb + kQGroup - 1) / kQGroup);
+      for (int g = 0; g < groups; ++g) {
+        const int slot = g % kQScaleSlots;
+        if (!__all_sync(0xffffffffu, q_wait(smem_u32(&bar_scale_full[slot]), (uint32_t)(g / kQScaleSlots) & 1u, &abort_flag))) {
+          if (lane == 0) report(p.t.status, 6, 1900 + slot, g);
+          break;
+        }
+        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_scale_full[slot]), 0));
+        __syncwarp();
       }
     }
   } else if (warp < 4) {
@@ -792,23 +788,23 @@ gemm_q_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
       decode_q_tile(t, p.t, mb, nb);
       const int first = for_q ? nb * 256 : mb * 256 + (int)rank * 128;
       for (int kb0 = 0; kb0 < num_kb; kb0 += kQGroup) {
-        uint32_t w[2][4];
+        // all loads of the group before the first use: one latency a group, and the slots let the warp run three groups ahead
+        uint32_t bits[2][4][kQGroup], w[2][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (h == 1 && !for_q) break;
-          uint32_t bits[4][kQGroup];
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float* src = o.s + scale_offset(o, first + h * 128 + i * 32 + lane) + (int64_t)kb0 * o.s_k;
 #pragma unroll
             for (int j = 0; j < kQGroup; ++j)
-              bits[i][j] = kb0 + j < num_kb ? __float_as_uint(__ldg(src + j * o.s_k)) : 0u;
+              bits[h][i][j] = (h == 0 || for_q) && kb0 + j < num_kb ? __float_as_uint(__ldg(src + j * o.s_k)) : 0u;
           }
 #pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
           for (int i = 0; i < 4; ++i)
-            w[h][i] = ((bits[i][0] >> 23) & 0xffu) | (((bits[i][1] >> 23) & 0xffu) << 8) | (((bits[i][2] >> 23) & 0xffu) << 16) |
-                      (((bits[i][3] >> 23) & 0xffu) << 24);
-        }
+            w[h][i] = ((bits[h][i][0] >> 23) & 0xffu) | (((bits[h][i][1] >> 23) & 0xffu) << 8) |
+                      (((bits[h][i][2] >> 23) & 0xffu) << 16) | (((bits[h][i][3] >> 23) & 0xffu) << 24);
         ok = __all_sync(0xffffffffu, q_wait(smem_u32(&bar_scale_empty[slot]), slot_phase ^ 1u, &abort_flag));
         if (!ok) {
           if (lane == 0) report(p.t.status, 3, 1700 + slot, kb0);
@@ -819,7 +815,7 @@ gemm_q_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
         if (for_q) dst[32] = make_uint4(w[1][0], w[1][1], w[1][2], w[1][3]);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // generic writes -> visible to the copy to TMEM
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_scale_full[slot]), 0));
+        if (lane == 0) mbar_arrive(smem_u32(&bar_scale_full[slot]));
         if (++slot == kQScaleSlots) { slot = 0; slot_phase ^= 1u; }
       }
     }
@@ -889,7 +885,8 @@ struct QSide {
   const float* s;
   int dim, k;        // extent of this side, contraction length
   int mn;            // stored [k, dim] instead of [dim, k]
-  int blocks;
+  int blocks;        // CLEAVE_BLOCKS_*
+  bool any_scales;   // not all of them powers of two
 };
 
 static bool side_map(CUtensorMap* map, const QSide& o, int box) {
@@ -991,7 +988,7 @@ static bool gemm_q_pairs(const QSide& a, const QSide& b, float* c, const float* 
 
 static bool gemm_q(const QSide& a, const QSide& b, float* c, const float* bias, int act) {
   const int64_t pair_tiles = (int64_t)ceil_div(a.dim, 256) * ceil_div(b.dim, 256);
-  if (pair_tiles >= ctx().sm_count / 4 && pair_tiles <= 0x3fffffff && a.dim > 128 && b.dim > 128)
+  if (!a.any_scales && !b.any_scales && pair_tiles >= ctx().sm_count / 4 && pair_tiles <= 0x3fffffff && a.dim > 128 && b.dim > 128)
     return gemm_q_pairs(a, b, c, bias, act);
   QGemmParams p = {};
   p.c = c;
@@ -1052,6 +1049,9 @@ int32_t cleave_cuda_gemm_e4m3(cleave_buf c, cleave_buf a, cleave_buf a_scale, in
   if (!q_operand(a, a_scale, ta ? k : m, ta ? m : k, a_blocks, "gemm_e4m3", &A) ||
       !q_operand(b, b_scale, tb ? n : k, tb ? k : n, b_blocks, "gemm_e4m3", &B))
     return -cleave_cuda_last_error();
+  const bool any_a = (a_blocks & CLEAVE_SCALES_ANY) != 0, any_b = (b_blocks & CLEAVE_SCALES_ANY) != 0;
+  a_blocks &= ~CLEAVE_SCALES_ANY;
+  b_blocks &= ~CLEAVE_SCALES_ANY;
   // A scale has to be constant over a k-block: vector blocks must run along the contraction.
   if (a_blocks == (ta ? CLEAVE_BLOCKS_ROWS : CLEAVE_BLOCKS_COLS) || b_blocks == (tb ? CLEAVE_BLOCKS_COLS : CLEAVE_BLOCKS_ROWS))
     return -set_error(CLEAVE_CUDA_ERR_ARG,
@@ -1076,7 +1076,7 @@ int32_t cleave_cuda_gemm_e4m3(cleave_buf c, cleave_buf a, cleave_buf a_scale, in
                           {bi ? bi->ptr : nullptr, bi ? bi->len * 4 : 0}};
   if (!ranges_distinct(out, 1, in, 5, "gemm_e4m3")) return -cleave_cuda_last_error();
   Trace tr("gemm_e4m3", "m=%d n=%d k=%d ta=%d tb=%d act=%d", m, n, k, ta, tb, act);
-  const QSide sa{A.q, A.s, m, k, ta, a_blocks}, sb{B.q, B.s, n, k, tb ? 0 : 1, b_blocks};
+  const QSide sa{A.q, A.s, m, k, ta, a_blocks, any_a}, sb{B.q, B.s, n, k, tb ? 0 : 1, b_blocks, any_b};
   return gemm_q(sa, sb, C->ptr, bi ? bi->ptr : nullptr, act) ? CLEAVE_CUDA_OK : -cleave_cuda_last_error();
 }
 

@@ -264,6 +264,7 @@ bool q_operand(cleave_buf q, cleave_buf s, int rows, int cols, int blocks, const
     set_error(CLEAVE_CUDA_ERR_ARG, "%s: rows and cols must be positive (got %d, %d)", what, rows, cols);
     return false;
   }
+  blocks &= ~CLEAVE_SCALES_ANY;
   if (blocks < CLEAVE_BLOCKS_ROWS || blocks > CLEAVE_BLOCKS_TILES) {
     set_error(CLEAVE_CUDA_ERR_ARG, "%s: unknown block form %d", what, blocks);
     return false;
@@ -417,6 +418,7 @@ int32_t cleave_cuda_dequantize_e4m3(cleave_buf out, cleave_buf q, cleave_buf s, 
   if (!O) return -cleave_cuda_last_error();
   QOperand in;
   if (!q_operand(q, s, rows, cols, blocks, "dequantize", &in)) return -cleave_cuda_last_error();
+  blocks &= ~CLEAVE_SCALES_ANY;
   if (O->len != (int64_t)rows * cols)
     return -set_error(CLEAVE_CUDA_ERR_SHAPE, "dequantize: output has %lld elements, not %d x %d", (long long)O->len, rows, cols);
   const MemRange outs[1] = {{O->ptr, O->len * 4}};
@@ -436,6 +438,7 @@ int32_t cleave_cuda_act_bwd_e4m3(cleave_buf y, cleave_buf y_scale, int32_t y_blo
   if (!ensure_init()) return -cleave_cuda_last_error();   // also makes the library's device this thread's
   QOperand Y;
   if (!q_operand(y, y_scale, rows, cols, y_blocks, "act_bwd", &Y)) return -cleave_cuda_last_error();
+  y_blocks &= ~CLEAVE_SCALES_ANY;
   Buf* G = as_buf(g, "act_bwd");
   if (!G) return -cleave_cuda_last_error();
   const int64_t n = (int64_t)rows * cols;

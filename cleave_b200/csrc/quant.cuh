@@ -5,8 +5,8 @@
 //   rows   1 x 128     scales [ceil(cols/128)][rows]
 //   cols   128 x 1     scales [ceil(rows/128)][cols]
 //   tiles  128 x 128   scales [ceil(rows/128)][ceil(cols/128)]
-// The value of an element is q * scale.  The quantizer's scales are powers of two, so that value is exact in f32 and
-// dividing by a scale loses nothing; the product accepts any finite scale.
+// The value of an element is q * scale.  The quantizer's scales are powers of two, so that value is exact in f32, dividing by
+// a scale loses nothing, and the tensor pipe can apply a scale by its exponent; CLEAVE_SCALES_ANY marks a tensor with others.
 #pragma once
 #include <stdint.h>
 

@@ -255,6 +255,7 @@ def gemm_into(c: Tensor, a: Tensor, b: Tensor, *, trans_a=False, trans_b=False, 
 
 # ---- 8-bit tensors with a scale per block of 128 ------------------------------------------------------------------
 BLOCKS = {"rows": 1, "cols": 2, "tiles": 3}
+SCALES_ANY = 16
 
 
 class QTensor:
@@ -263,15 +264,16 @@ class QTensor:
     ``blocks`` says which elements share a scale: ``"rows"`` 1 x 128 (an operand whose contraction runs along its rows),
     ``"cols"`` 128 x 1 (... down its columns), ``"tiles"`` 128 x 128 (weights: either way).  ``scales`` is an f32
     ``Tensor`` [ceil(cols/128), rows], [ceil(rows/128), cols] or [ceil(rows/128), ceil(cols/128)].  The bytes are
-    row-major with a row pitch of ``cols`` rounded up to 16.
+    row-major with a row pitch of ``cols`` rounded up to 16.  Scales are powers of two unless ``any_scales`` says otherwise.
     """
 
-    __slots__ = ("_h", "scales", "dims", "blocks")
+    __slots__ = ("_h", "scales", "dims", "blocks", "any_scales")
 
-    def __init__(self, rows: int, cols: int, blocks: str, *, _handle=None, _scales: Tensor | None = None):
+    def __init__(self, rows: int, cols: int, blocks: str, *, any_scales: bool = False, _handle=None,
+                 _scales: Tensor | None = None):
         """An uninitialised 8-bit tensor, the destination of ``quantize_into`` / ``nn.act_bwd_q``."""
         self._h = None
-        self.dims, self.blocks = _q_dims(rows, cols, blocks), blocks
+        self.dims, self.blocks, self.any_scales = _q_dims(rows, cols, blocks), blocks, bool(any_scales)
         if _handle is None:
             _handle = lib().cleave_cuda_alloc_e4m3(self.nbytes)
             if not _handle:
@@ -280,8 +282,9 @@ class QTensor:
         self.scales = _scales if _scales is not None else Tensor.empty(*self.scale_dims)
 
     @classmethod
-    def from_device_ptr(cls, ptr: int, scales_ptr: int, rows: int, cols: int, blocks: str) -> "QTensor":
-        """Non-owning view of caller-owned device memory: the bytes (16-byte aligned, pitch as above) and the scales."""
+    def from_device_ptr(cls, ptr: int, scales_ptr: int, rows: int, cols: int, blocks: str, any_scales: bool = False) -> "QTensor":
+        """Non-owning view of caller-owned device memory: the bytes (16-byte aligned, pitch as above) and the scales.
+        ``any_scales`` has to be set where they are not all positive powers of two: nothing looks at them here."""
         dims = _q_dims(rows, cols, blocks)
         h = lib().cleave_cuda_wrap_e4m3(ctypes.c_void_p(ptr), lib().cleave_cuda_e4m3_bytes(*dims))
         if not h:
@@ -291,22 +294,29 @@ class QTensor:
         except Exception:
             lib().cleave_cuda_free(h)
             raise
-        return cls(rows, cols, blocks, _handle=h, _scales=scales)
+        return cls(rows, cols, blocks, any_scales=any_scales, _handle=h, _scales=scales)
 
     @classmethod
     def from_numpy(cls, data: np.ndarray, scales: np.ndarray, cols: int, blocks: str) -> "QTensor":
-        """Uploads e4m3 bytes [rows, pitch] (uint8) and their scales."""
+        """Uploads e4m3 bytes [rows, pitch] (uint8) and their scales, and sets ``any_scales`` as they are."""
         data = np.ascontiguousarray(data, np.uint8)
         if data.ndim != 2:
             raise TypeError("QTensor: the bytes are a [rows, pitch] array")
         dims = _q_dims(data.shape[0], cols, blocks)
         if data.size != lib().cleave_cuda_e4m3_bytes(*dims) or tuple(np.shape(scales)) != _scale_dims(dims, blocks):
             raise TypeError(f"QTensor: bytes {data.shape} and scales {np.shape(scales)} are not those of {dims}, {blocks!r}")
+        half, exponent = np.frexp(np.asarray(scales, np.float32))
+        powers = bool(np.all((half == 0.5) & (exponent > -126)))
         s = Tensor(scales)
         h = lib().cleave_cuda_upload_e4m3(data.ctypes.data_as(c_u8p), data.size)
         if not h:
             raise_last_error("QTensor upload")
-        return cls(*dims, blocks, _handle=h, _scales=s)
+        return cls(*dims, blocks, any_scales=not powers, _handle=h, _scales=s)
+
+    @property
+    def form(self) -> int:
+        """The block form as the C ABI spells it."""
+        return BLOCKS[self.blocks] | (SCALES_ANY if self.any_scales else 0)
 
     @property
     def nbytes(self) -> int:
@@ -389,7 +399,7 @@ def dequantize(q: QTensor, out: Tensor | None = None) -> Tensor:
     if out is not None and (out.dims != q.dims or out.dtype != "f32"):
         raise TypeError(f"dequantize: cannot write {q!r} into {out!r}")
     out = out if out is not None else Tensor.empty(*q.dims)
-    if lib().cleave_cuda_dequantize_e4m3(out._h, q._h, q.scales._h, *q.dims, BLOCKS[q.blocks]) != 0:
+    if lib().cleave_cuda_dequantize_e4m3(out._h, q._h, q.scales._h, *q.dims, q.form) != 0:
         raise_last_error("dequantize")
     return out
 
@@ -410,7 +420,7 @@ def gemm_q_into(c: Tensor, a: QTensor, b: QTensor, *, trans_a=False, trans_b=Fal
                         f"{b!r} (trans_b={bool(trans_b)})")
     if bias is not None and bias.dims != (n,):
         raise TypeError(f"gemm_q_into: bias {bias!r} for {n} columns")
-    if lib().cleave_cuda_gemm_e4m3(c._h, a._h, a.scales._h, BLOCKS[a.blocks], b._h, b.scales._h, BLOCKS[b.blocks], m, n, k,
+    if lib().cleave_cuda_gemm_e4m3(c._h, a._h, a.scales._h, a.form, b._h, b.scales._h, b.form, m, n, k,
                                    int(trans_a), int(trans_b), bias._h if bias is not None else None, ACT[act]) != 0:
         raise_last_error("gemm_q_into")
     return c

@@ -12,7 +12,7 @@ from __future__ import annotations
 import math
 
 from ._lib import lib, raise_last_error
-from .linalg import ACT, BLOCKS, QTensor, Tensor, _q_handles, _q_outputs
+from .linalg import ACT, QTensor, Tensor, _q_handles, _q_outputs
 
 
 def _unary(what: str):
@@ -75,7 +75,7 @@ def act_bwd_q(y: QTensor, g: Tensor, act: str, *outs: QTensor, dz: Tensor | None
     if not got and dz is None and db is None:
         raise TypeError("act_bwd_q: no output given")
     h = lambda t: t._h if t is not None else None  # noqa: E731
-    if lib().cleave_cuda_act_bwd_e4m3(y._h, y.scales._h, BLOCKS[y.blocks], g._h, *y.dims, ACT[act], h(dz),
+    if lib().cleave_cuda_act_bwd_e4m3(y._h, y.scales._h, y.form, g._h, *y.dims, ACT[act], h(dz),
                                       *_q_handles(got, "rows"), *_q_handles(got, "cols"), h(db)) != 0:
         raise_last_error("act_bwd_q")
 

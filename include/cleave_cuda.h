@@ -365,8 +365,12 @@ int32_t cleave_cuda_sgd_f64(cleave_buf w, cleave_buf g, double lr, double gscale
  *   ROWS    1 x 128     scales [ceil(cols/128)][rows]            an operand whose contraction runs along a row
  *   COLS    128 x 1     scales [ceil(rows/128)][cols]            an operand whose contraction runs down a column
  *   TILES   128 x 128   scales [ceil(rows/128)][ceil(cols/128)]  weights: either way
- * Blocks at the right and lower edge are what is left of the matrix. */
-enum { CLEAVE_BLOCKS_ROWS = 1, CLEAVE_BLOCKS_COLS = 2, CLEAVE_BLOCKS_TILES = 3 };
+ * Blocks at the right and lower edge are what is left of the matrix.
+ * Scales are positive powers of two, 2^-126 to 2^127, as cleave_cuda_quantize_e4m3 makes them: large products let the
+ * tensor pipe apply them, which reads nothing but a scale's exponent.  A tensor from elsewhere whose scales are other f32
+ * values is marked by adding CLEAVE_SCALES_ANY to its block form wherever it is read; its large products take the kernel that
+ * multiplies by the scales (about half as fast). */
+enum { CLEAVE_BLOCKS_ROWS = 1, CLEAVE_BLOCKS_COLS = 2, CLEAVE_BLOCKS_TILES = 3, CLEAVE_SCALES_ANY = 16 };
 int64_t cleave_cuda_e4m3_bytes(int32_t rows, int32_t cols);                     /* length of the byte handle */
 int64_t cleave_cuda_e4m3_scales(int32_t rows, int32_t cols, int32_t blocks);    /* length of the scale handle */
 cleave_buf cleave_cuda_alloc_e4m3(int64_t bytes);                               /* uninitialised */
@@ -383,7 +387,7 @@ int32_t cleave_cuda_quantize_e4m3(cleave_buf x, int32_t rows, int32_t cols, clea
 int32_t cleave_cuda_dequantize_e4m3(cleave_buf out, cleave_buf q, cleave_buf s, int32_t rows, int32_t cols, int32_t blocks);
 /* c[m, n] = act(op(A) * op(B) + bias), all sums in f32.  Stored layouts as in cleave_cuda_gemm_ex_f32: A [m,k] ([k,m] if
  * trans_a), B [k,n] ([n,k] if trans_b).  Blocks run along the contraction or are tiles: A ROWS (COLS if trans_a) or TILES,
- * B COLS (ROWS if trans_b) or TILES; scales may be any finite f32 values.  bias may be NULL (n elements otherwise).  Any
+ * B COLS (ROWS if trans_b) or TILES, each plus CLEAVE_SCALES_ANY where its scales are not powers of two.  bias may be NULL (n elements otherwise).  Any
  * size from 1 up.  A layer's products: X W (X ROWS, W TILES), dZ W^T (dZ ROWS, W TILES, trans_b), X^T dZ (both COLS,
  * trans_a).  The result is reproducible run to run. */
 int32_t cleave_cuda_gemm_e4m3(cleave_buf c, cleave_buf a, cleave_buf a_scale, int32_t a_blocks, cleave_buf b,

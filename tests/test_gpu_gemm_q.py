@@ -1,10 +1,12 @@
 """The block-scaled 8-bit product against 64-bit products of the values the operands stand for.
 
-Error bound of an element, with S = sum over k of |a| |b| (the values): inside a k-block the tensor pipe adds up to 128
-exact products into an f32 accumulator that truncates, at most 2^-23 of a partial sum each, so at most 128 * 2^-23 of the block's part
-of S; the two scales' product and its product with the block sum round three times, 3 * 2^-24; the running sum adds at most
-2^-24 of S per k-block and per rank of a split.  Together (128 * 2 + 3 + blocks + 8) * 2^-24 * S.  The bias adds 2^-24 of the
-result, an activation is a contraction (slope at most 1) evaluated to within 4e-7 of its value (absolute for tanh)."""
+Error bound of an element, with S = sum over k of |a| |b| (the values).  The tensor pipe adds 32 exact products at a time into
+an f32 accumulator that truncates, so at most 2^-23 of a partial sum per term summed there; it runs over at most 1024 terms
+(eight k-blocks; one where the kernel scales them itself) before it is added to a running sum.  Taking every one of a k-block's
+128 terms as an add of its own, as if it were the worst of them, covers the 32 adds of 1024 terms four times over: 128 * 2^-23 of
+S.  Where the kernel scales, the scales' product and its product with the block's sum round three times, 3 * 2^-24; the
+running sum adds at most 2^-24 of S per k-block and per rank of a split.  Together (128 * 2 + 3 + blocks + 8) * 2^-24 * S.  The
+bias adds 2^-24 of the result, an activation is a contraction (slope at most 1) evaluated to within 4e-7 of its value."""
 import ctypes
 
 import numpy as np
@@ -106,17 +108,39 @@ def scaled(t: QTensor, factor: float) -> QTensor:
     return QTensor.from_numpy(t.numpy(), t.scales.numpy() * f32(factor), t.dims[1], t.blocks)
 
 
-def test_scales_may_be_any_values():
+@pytest.mark.parametrize("m,n,k", [(70, 190, 500), (3, 700, 900), (1540, 1700, 260)])
+def test_scales_may_be_any_values(m, n, k):
     rng = np.random.default_rng(9)
-    m, n, k = 70, 190, 500
     a, _ = operand(6, m, k, False, "rows")
     b, _ = operand(7, n, k, False, "rows")
     sa, sb = rng.uniform(0.1, 3, a.scale_dims).astype(f32), rng.uniform(-2, 2, b.scale_dims).astype(f32)
     qa, qb = a.numpy(), b.numpy()
     av, bv = qr.values(qa, sa, "rows", k), qr.values(qb, sb, "rows", k)
-    c = linalg.gemm_q_into(Tensor.empty(m, n), QTensor.from_numpy(qa, sa, k, "rows"), QTensor.from_numpy(qb, sb, k, "rows"),
-                           trans_b=True).numpy()
+    ta, tb = QTensor.from_numpy(qa, sa, k, "rows"), QTensor.from_numpy(qb, sb, k, "rows")
+    assert ta.any_scales and tb.any_scales and not a.any_scales
+    c = linalg.gemm_q_into(Tensor.empty(m, n), ta, tb, trans_b=True).numpy()
     assert np.all(np.abs(c - av @ bv.T) <= bound(av, bv))
+    # one operand of each kind
+    c = linalg.gemm_q_into(Tensor.empty(m, n), a, tb, trans_b=True).numpy()
+    av = qr.values(qa, a.scales.numpy(), "rows", k)
+    assert np.all(np.abs(c - av @ bv.T) <= bound(av, bv))
+    # and read back
+    assert np.array_equal(linalg.dequantize(tb).numpy(), (qr.TABLE[qb[:, :k]].astype(f32) * qr.spread(sb, "rows", n, k)))
+
+
+@pytest.mark.parametrize("m,n,k", [(65, 130, 1500), (1540, 1700, 700)])
+def test_scales_far_apart(m, n, k):
+    # scales from one end of the range of powers of two to the other, in one sum and in one product
+    rng = np.random.default_rng(19)
+    a, _ = operand(6, m, k, False, "rows")
+    b, _ = operand(7, n, k, False, "rows")
+    sa = (2.0 ** rng.integers(-100, 60, a.scale_dims)).astype(f32)
+    sb = (2.0 ** rng.integers(-20, 40, b.scale_dims)).astype(f32)
+    ta, tb = QTensor.from_numpy(a.numpy(), sa, k, "rows"), QTensor.from_numpy(b.numpy(), sb, k, "rows")
+    assert not ta.any_scales and not tb.any_scales
+    av, bv = qr.values(a.numpy(), sa, "rows", k), qr.values(b.numpy(), sb, "rows", k)
+    c = linalg.gemm_q_into(Tensor.empty(m, n), ta, tb, trans_b=True).numpy()
+    assert np.all(np.abs(c - av @ bv.T) <= bound(av, bv) + 1e-37)
 
 
 def test_nan_reaches_its_row_and_no_other():
