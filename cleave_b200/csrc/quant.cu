@@ -1,9 +1,9 @@
 // Block quantization to 8 bits, its inverse, and the derivative form of an activation that was kept in 8 bits.
 //
-// One kernel does all the writing.  A CTA takes a 128 x 128 tile, one block of every form, holds it in registers (64 values a
-// thread, loaded as 16 independent 16-byte words) and makes each form that is asked for from that one read: a warp owns 16
+// One kernel does all the writing.  A CTA takes a 128 x 128 tile, one block of every form, holds it in registers (32 values a
+// thread, all its loads issued before the first use) and makes each form that is asked for from that one read: a warp owns 8
 // whole rows of the tile, so a 1 x 128 block's maximum is one warp reduction, and a 128 x 1 block's is a maximum over the
-// warp's 16 rows in a register and over the 8 warps in shared memory.  HBM bound: 4 bytes read (5 with a checkpoint) and one
+// warp's 8 rows in a register and over the 16 warps in shared memory.  HBM bound: 4 bytes read (5 with a checkpoint) and one
 // byte written per element and form.
 //
 // Scale of a block: s = 2^e with e = ceil(log2(amax / 448)), the smallest power of two that brings the block's largest
@@ -21,9 +21,10 @@
 
 namespace cleave {
 
-constexpr int kQThreads = 256;
+constexpr int kQThreads = 512;
 constexpr int kQWarps = kQThreads / 32;
 constexpr int kQRows = kQBlock / kQWarps;   // rows of the tile per warp
+constexpr int kQMaxColBlocks = 4096;        // column sums finished in the kernel up to this many
 
 struct TileArgs {
   int rows, cols;
@@ -36,15 +37,14 @@ struct TileArgs {
   uint8_t *q_rows, *q_cols, *q_tiles;
   float *s_rows, *s_cols, *s_tiles;
   float* db_part;         // [row blocks][cols]: column sums of each row block
+  float* db;              // their sum, written by the last CTA of each column block (null: left to a second kernel)
 };
 
-// |v| as an ordered integer; 0 for a non-finite v.
-__device__ __forceinline__ uint32_t finite_abs_bits(float v) {
-  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-  return b < 0x7f800000u ? b : 0u;
-}
+// Arrivals of a column block's CTAs; each count wraps to zero with the last arrival.  Launches of this library are ordered on
+// one stream, so no two of them count at once.
+static __device__ unsigned int g_db_arrivals[kQMaxColBlocks];
 
-// Biased exponent of the block's scale, in [1, 247].
+// Biased exponent of the block's scale, in [1, 247], from the bits of its largest magnitude.
 __device__ __forceinline__ uint32_t scale_exponent(uint32_t amax_bits) {
   const int e = (int)((amax_bits + 0x1fffffu) >> 23) - 8;   // E - 8 (biased), + 1 where the mantissa is above 1.75's
   return (uint32_t)(e < 1 ? 1 : e);
@@ -52,17 +52,18 @@ __device__ __forceinline__ uint32_t scale_exponent(uint32_t amax_bits) {
 __device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float(e << 23); }
 __device__ __forceinline__ float inverse_scale_of(uint32_t e) { return __uint_as_float((254u - e) << 23); }
 
-// Two values to two e4m3 bytes (lo in the low byte), round to nearest even.
+// v with an infinity turned into NaN (v * 0 is a zero of v's sign, or NaN), which maxima then skip and conversions keep.
+__device__ __forceinline__ float finite_or_nan(float v) { return __fmaf_rn(v, 0.0f, v); }
+
+// Two values to two e4m3 bytes (lo in the low byte), round to nearest even; NaN to 0x7F.
 __device__ __forceinline__ uint32_t e4m3x2(float hi, float lo) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ float scaled(float v, float inv) {
-  return finite_abs_bits(v) == 0u && v != 0.0f ? __uint_as_float(0x7fc00000u) : __fmul_rn(v, inv);
-}
 __device__ __forceinline__ uint32_t quantize4(const float (&v)[4], const float (&inv)[4]) {
-  return e4m3x2(scaled(v[1], inv[1]), scaled(v[0], inv[0])) | (e4m3x2(scaled(v[3], inv[3]), scaled(v[2], inv[2])) << 16);
+  return e4m3x2(__fmul_rn(v[1], inv[1]), __fmul_rn(v[0], inv[0])) |
+         (e4m3x2(__fmul_rn(v[3], inv[3]), __fmul_rn(v[2], inv[2])) << 16);
 }
 // Four e4m3 bytes to f32 (exact).
 __device__ __forceinline__ void unpack4(uint32_t w, float (&v)[4]) {
@@ -85,145 +86,177 @@ __device__ __forceinline__ float act_grad(float y, float g, int act) {
 
 template <bool CHECKPOINT>
 __global__ void __launch_bounds__(kQThreads, 2) tile_kernel(const TileArgs a) {
-  __shared__ uint32_t s_max[kQWarps][kQBlock];
-  __shared__ float s_sum[kQWarps][kQBlock];
+  __shared__ float s_max[kQWarps][kQBlock];
+  __shared__ float s_sum[CHECKPOINT ? kQWarps : 1][kQBlock];
+  __shared__ bool s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int col_blocks = (a.cols + kQBlock - 1) / kQBlock;
   const int rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
   const int r0 = rb * kQBlock + warp * kQRows, c0 = cb * kQBlock + lane * 4;
   const int64_t pitch = ((int64_t)a.cols + 15) / 16 * 16;
+  const int rows_here = a.rows - r0 < kQRows ? a.rows - r0 : kQRows;   // may be negative
 
+  // ---- every load of the thread
   float v[kQRows][4];
+  const float* src = a.x + (int64_t)r0 * a.cols + c0;
+  if (a.vec) {
 #pragma unroll
-  for (int i = 0; i < kQRows; ++i) {
-    const int r = r0 + i;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[i][j] = 0.0f;
-    if (r < a.rows) {
-      const float* src = a.x + (int64_t)r * a.cols + c0;
-      if (a.vec) {
-        if (c0 < a.cols) {
-          const float4 t = __ldcs(reinterpret_cast<const float4*>(src));
-          v[i][0] = t.x; v[i][1] = t.y; v[i][2] = t.z; v[i][3] = t.w;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c0 + j < a.cols) v[i][j] = __ldg(src + j);
-      }
+    for (int i = 0; i < kQRows; ++i) {
+      float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (i < rows_here && c0 < a.cols) t = __ldcs(reinterpret_cast<const float4*>(src + (int64_t)i * a.cols));
+      v[i][0] = t.x; v[i][1] = t.y; v[i][2] = t.z; v[i][3] = t.w;
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kQRows; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = i < rows_here && c0 + j < a.cols ? __ldg(src + (int64_t)i * a.cols + j) : 0.0f;
   }
   if constexpr (CHECKPOINT) {
-    float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    uint32_t w[kQRows];
+    const uint8_t* ysrc = a.y_q + r0 * pitch + c0;
+#pragma unroll
+    for (int i = 0; i < kQRows; ++i)
+      w[i] = i < rows_here && c0 < a.cols ? __ldcs(reinterpret_cast<const uint32_t*>(ysrc + i * pitch)) : 0u;
+    float sc[4];
+    float row_scale = 0.0f;   // ROWS: lane i holds row i's
     if (a.y_blocks == CLEAVE_BLOCKS_COLS) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (c0 + j < a.cols) sc[j] = __ldg(a.y_s + (int64_t)rb * a.cols + c0 + j);
+      for (int j = 0; j < 4; ++j) sc[j] = c0 + j < a.cols ? __ldg(a.y_s + (int64_t)rb * a.cols + c0 + j) : 0.0f;
     } else if (a.y_blocks == CLEAVE_BLOCKS_TILES) {
       sc[0] = sc[1] = sc[2] = sc[3] = __ldg(a.y_s + (int64_t)rb * col_blocks + cb);
+    } else {
+      if (lane < rows_here) row_scale = __ldg(a.y_s + (int64_t)cb * a.rows + r0 + lane);
     }
 #pragma unroll
     for (int i = 0; i < kQRows; ++i) {
-      const int r = r0 + i;
-      if (r < a.rows && c0 < a.cols) {
-        const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(a.y_q + r * pitch + c0));
-        if (a.y_blocks == CLEAVE_BLOCKS_ROWS) sc[0] = sc[1] = sc[2] = sc[3] = __ldg(a.y_s + (int64_t)cb * a.rows + r);
-        float y[4];
-        unpack4(w, y);
+      float y[4];
+      unpack4(w[i], y);
+      if (a.y_blocks == CLEAVE_BLOCKS_ROWS) sc[0] = sc[1] = sc[2] = sc[3] = __shfl_sync(0xffffffffu, row_scale, i);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          v[i][j] = c0 + j < a.cols ? act_grad(__fmul_rn(y[j], sc[j]), v[i][j], a.act) : 0.0f;   // padding bytes may be anything
-      }
+      for (int j = 0; j < 4; ++j)
+        v[i][j] = i < rows_here && c0 + j < a.cols ? act_grad(__fmul_rn(y[j], sc[j]), v[i][j], a.act) : 0.0f;   // padding bytes may be anything
     }
     if (a.dz != nullptr) {
+      float* dst = a.dz + (int64_t)r0 * a.cols + c0;
 #pragma unroll
       for (int i = 0; i < kQRows; ++i) {
-        const int r = r0 + i;
-        if (r < a.rows) {
-          float* dst = a.dz + (int64_t)r * a.cols + c0;
-          if (a.vec) {
-            if (c0 < a.cols) *reinterpret_cast<float4*>(dst) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
-          } else {
+        if (i >= rows_here) break;
+        if (a.vec) {
+          if (c0 < a.cols) __stcs(reinterpret_cast<float4*>(dst + (int64_t)i * a.cols), make_float4(v[i][0], v[i][1], v[i][2], v[i][3]));
+        } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (c0 + j < a.cols) dst[j] = v[i][j];
-          }
+          for (int j = 0; j < 4; ++j)
+            if (c0 + j < a.cols) dst[(int64_t)i * a.cols + j] = v[i][j];
         }
       }
     }
-  }
-
-  // ---- 1 x 128 blocks: a row of the tile is one warp's
-  if (a.q_rows != nullptr) {
-    float own_scale = 0.0f;
+    if (a.db_part != nullptr) {
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < kQRows; ++i) {
-      uint32_t m = 0;
+      for (int i = 0; i < kQRows; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) m = max(m, finite_abs_bits(v[i][j]));
-      const uint32_t e = scale_exponent(__reduce_max_sync(0xffffffffu, m));
-      if (lane == i) own_scale = scale_of(e);
-      const float inv = inverse_scale_of(e);
-      const float inv4[4] = {inv, inv, inv, inv};
-      const int r = r0 + i;
-      if (r < a.rows && c0 < pitch) *reinterpret_cast<uint32_t*>(a.q_rows + r * pitch + c0) = quantize4(v[i], inv4);
+        for (int j = 0; j < 4; ++j) sum[j] = __fadd_rn(sum[j], v[i][j]);
+      *reinterpret_cast<float4*>(&s_sum[warp][lane * 4]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
     }
-    if (lane < kQRows && r0 + lane < a.rows) a.s_rows[(int64_t)cb * a.rows + r0 + lane] = own_scale;
   }
-
-  // ---- what needs the whole tile: column maxima, the tile's maximum, column sums
-  if (a.q_cols == nullptr && a.q_tiles == nullptr && a.db_part == nullptr) return;
-  uint32_t m[4] = {0, 0, 0, 0};
-  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < kQRows; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      m[j] = max(m[j], finite_abs_bits(v[i][j]));
-      sum[j] = __fadd_rn(sum[j], v[i][j]);
-    }
-  *reinterpret_cast<uint4*>(&s_max[warp][lane * 4]) = make_uint4(m[0], m[1], m[2], m[3]);
-  *reinterpret_cast<float4*>(&s_sum[warp][lane * 4]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
-  __syncthreads();
-  if (a.db_part != nullptr && threadIdx.x < kQBlock) {
-    const int c = cb * kQBlock + (int)threadIdx.x;
-    if (c < a.cols) {
-      float t = s_sum[0][threadIdx.x];
+    for (int j = 0; j < 4; ++j) v[i][j] = finite_or_nan(v[i][j]);
+  const bool in_pitch = c0 < pitch;   // the padding behind the last column gets zeros
+
+  // ---- column maxima to shared memory
+  const bool whole_tile = a.q_cols != nullptr || a.q_tiles != nullptr;
+  if (whole_tile) {
+    float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int w = 1; w < kQWarps; ++w) t = __fadd_rn(t, s_sum[w][threadIdx.x]);
+    for (int i = 0; i < kQRows; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], fabsf(v[i][j]));
+    *reinterpret_cast<float4*>(&s_max[warp][lane * 4]) = make_float4(m[0], m[1], m[2], m[3]);
+  }
+  // ---- 1 x 128 blocks: a row of the tile is one warp's
+  if (a.q_rows != nullptr) {
+    float own_scale = 0.0f;
+    uint8_t* dst = a.q_rows + r0 * pitch + c0;
+#pragma unroll
+    for (int i = 0; i < kQRows; ++i) {
+      const float m = fmaxf(fmaxf(fmaxf(0.0f, fabsf(v[i][0])), fabsf(v[i][1])), fmaxf(fmaxf(0.0f, fabsf(v[i][2])), fabsf(v[i][3])));
+      const uint32_t e = scale_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+      if (lane == i) own_scale = scale_of(e);
+      const float inv = inverse_scale_of(e);
+      const float inv4[4] = {inv, inv, inv, inv};
+      if (i < rows_here && in_pitch) *reinterpret_cast<uint32_t*>(dst + i * pitch) = quantize4(v[i], inv4);
+    }
+    if (lane < rows_here && lane < kQRows) a.s_rows[(int64_t)cb * a.rows + r0 + lane] = own_scale;
+  }
+  if (!whole_tile && (!CHECKPOINT || a.db_part == nullptr)) return;
+  __syncthreads();
+  if (whole_tile) {
+    float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kQWarps; ++w) {
+      const float4 t = *reinterpret_cast<const float4*>(&s_max[w][lane * 4]);
+      m[0] = fmaxf(m[0], t.x); m[1] = fmaxf(m[1], t.y); m[2] = fmaxf(m[2], t.z); m[3] = fmaxf(m[3], t.w);
+    }
+    if (a.q_cols != nullptr) {
+      float inv[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t e = scale_exponent(__float_as_uint(m[j]));
+        inv[j] = inverse_scale_of(e);
+        if (warp == 0 && c0 + j < a.cols) a.s_cols[(int64_t)rb * a.cols + c0 + j] = scale_of(e);
+      }
+      uint8_t* dst = a.q_cols + r0 * pitch + c0;
+#pragma unroll
+      for (int i = 0; i < kQRows; ++i)
+        if (i < rows_here && in_pitch) *reinterpret_cast<uint32_t*>(dst + i * pitch) = quantize4(v[i], inv);
+    }
+    if (a.q_tiles != nullptr) {
+      const uint32_t e = scale_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])))));
+      const float inv = inverse_scale_of(e);
+      const float inv4[4] = {inv, inv, inv, inv};
+      if (threadIdx.x == 0) a.s_tiles[(int64_t)rb * col_blocks + cb] = scale_of(e);
+      uint8_t* dst = a.q_tiles + r0 * pitch + c0;
+#pragma unroll
+      for (int i = 0; i < kQRows; ++i)
+        if (i < rows_here && in_pitch) *reinterpret_cast<uint32_t*>(dst + i * pitch) = quantize4(v[i], inv4);
+    }
+  }
+  if constexpr (CHECKPOINT) {
+    // ---- column sums: of the tile, then, by the last CTA of the column block to get here, of the row blocks in ascending
+    // order, four runs of them side by side: the order of the additions is a function of the shape alone
+    if (a.db_part == nullptr) return;
+    const int tc = threadIdx.x & (kQBlock - 1), part = threadIdx.x / kQBlock;   // column, one of four
+    const int c = cb * kQBlock + tc;
+    if (part == 0 && c < a.cols) {
+      float t = s_sum[0][tc];
+#pragma unroll
+      for (int w = 1; w < kQWarps; ++w) t = __fadd_rn(t, s_sum[w][tc]);
       a.db_part[(int64_t)rb * a.cols + c] = t;
     }
-  }
-  if (a.q_cols == nullptr && a.q_tiles == nullptr) return;
-#pragma unroll
-  for (int w = 0; w < kQWarps; ++w) {
-    const uint4 t = *reinterpret_cast<const uint4*>(&s_max[w][lane * 4]);
-    m[0] = max(m[0], t.x); m[1] = max(m[1], t.y); m[2] = max(m[2], t.z); m[3] = max(m[3], t.w);
-  }
-  if (a.q_cols != nullptr) {
-    float inv[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t e = scale_exponent(m[j]);
-      inv[j] = inverse_scale_of(e);
-      if (warp == 0 && c0 + j < a.cols) a.s_cols[(int64_t)rb * a.cols + c0 + j] = scale_of(e);
+    if (a.db == nullptr) return;
+    const int row_blocks = (a.rows + kQBlock - 1) / kQBlock;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      unsigned int before;
+      asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;"
+                   : "=r"(before) : "l"(&g_db_arrivals[cb]), "r"((unsigned int)(row_blocks - 1)) : "memory");
+      s_last = before == (unsigned int)(row_blocks - 1);
     }
-#pragma unroll
-    for (int i = 0; i < kQRows; ++i) {
-      const int r = r0 + i;
-      if (r < a.rows && c0 < pitch) *reinterpret_cast<uint32_t*>(a.q_cols + r * pitch + c0) = quantize4(v[i], inv);
-    }
-  }
-  if (a.q_tiles != nullptr) {
-    const uint32_t e = scale_exponent(__reduce_max_sync(0xffffffffu, max(max(m[0], m[1]), max(m[2], m[3]))));
-    const float inv = inverse_scale_of(e);
-    const float inv4[4] = {inv, inv, inv, inv};
-    if (threadIdx.x == 0) a.s_tiles[(int64_t)rb * col_blocks + cb] = scale_of(e);
-#pragma unroll
-    for (int i = 0; i < kQRows; ++i) {
-      const int r = r0 + i;
-      if (r < a.rows && c0 < pitch) *reinterpret_cast<uint32_t*>(a.q_tiles + r * pitch + c0) = quantize4(v[i], inv4);
-    }
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    const int per = (row_blocks + 3) / 4, first = part * per;
+    float t = 0.0f;
+    if (c < a.cols)
+      for (int r = first; r < first + per && r < row_blocks; ++r) t = __fadd_rn(t, __ldcg(a.db_part + (int64_t)r * a.cols + c));
+    s_sum[part][tc] = t;
+    __syncthreads();
+    if (part == 0 && c < a.cols)
+      a.db[c] = __fadd_rn(__fadd_rn(s_sum[0][tc], s_sum[1][tc]), __fadd_rn(s_sum[2][tc], s_sum[3][tc]));
   }
 }
 
@@ -488,17 +521,20 @@ int32_t cleave_cuda_act_bwd_e4m3(cleave_buf y, cleave_buf y_scale, int32_t y_blo
   a.dz = DZ ? DZ->ptr : nullptr;
   a.q_rows = o[0].q; a.s_rows = o[0].s;
   a.q_cols = o[1].q; a.s_cols = o[1].s;
-  // Column sums: every tile leaves the sums of its 128 rows, a second pass adds the row blocks in ascending order.
+  // Column sums: every tile leaves the sums of its 128 rows; the kernel adds the row blocks itself, or, where there are more
+  // column blocks than counters, a second one does.
   const int row_blocks = ceil_div(rows, kQBlock);
+  const bool in_kernel = ceil_div(cols, kQBlock) <= kQMaxColBlocks;
   float* part = nullptr;
   if (DB) {
     part = row_blocks == 1 ? DB->ptr : scratch_alloc((int64_t)row_blocks * cols * (int64_t)sizeof(float));
     if (!part) return -cleave_cuda_last_error();
     a.db_part = part;
+    a.db = row_blocks > 1 && in_kernel ? DB->ptr : nullptr;
   }
   bool ok = launch_tiles(a, "act_bwd");
   if (DB && row_blocks > 1) {
-    ok = ok && colsum_launch(part, DB->ptr, row_blocks, cols, ctx().stream);
+    if (!in_kernel) ok = ok && colsum_launch(part, DB->ptr, row_blocks, cols, ctx().stream);
     scratch_free(part);
   }
   return ok ? CLEAVE_CUDA_OK : -cleave_cuda_last_error();
