@@ -44,13 +44,14 @@ struct TileArgs {
 // one stream, so no two of them count at once.
 static __device__ unsigned int g_db_arrivals[kQMaxColBlocks];
 
-// Biased exponent of the block's scale, in [1, 247], from the bits of its largest magnitude.
-__device__ __forceinline__ uint32_t scale_exponent(uint32_t amax_bits) {
-  const int e = (int)((amax_bits + 0x1fffffu) >> 23) - 8;   // E - 8 (biased), + 1 where the mantissa is above 1.75's
-  return (uint32_t)(e < 1 ? 1 : e);
+// Exponent field of a block's largest magnitude after the carry described above, held at 9 or more (a scale of 2^-126);
+// scale and 1 / scale follow by one subtraction each.
+__device__ __forceinline__ uint32_t amax_exponent(uint32_t amax_bits) {
+  const uint32_t e = (amax_bits + 0x1fffffu) & 0x7f800000u;
+  return e < (9u << 23) ? 9u << 23 : e;
 }
-__device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float(e << 23); }
-__device__ __forceinline__ float inverse_scale_of(uint32_t e) { return __uint_as_float((254u - e) << 23); }
+__device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float(e - (8u << 23)); }
+__device__ __forceinline__ float inverse_scale_of(uint32_t e) { return __uint_as_float((262u << 23) - e); }
 
 // v with an infinity turned into NaN (v * 0 is a zero of v's sign, or NaN), which maxima then skip and conversions keep.
 __device__ __forceinline__ float finite_or_nan(float v) { return __fmaf_rn(v, 0.0f, v); }
@@ -75,35 +76,43 @@ __device__ __forceinline__ void unpack4(uint32_t w, float (&v)[4]) {
 }
 
 // act'(y) * g with every step rounded as the f32 derivative forms round it (elementwise.cu).
-__device__ __forceinline__ float act_grad(float y, float g, int act) {
-  switch (act) {
-    case CLEAVE_ACT_TANH: return __fmul_rn(__fsub_rn(1.0f, __fmul_rn(y, y)), g);
-    case CLEAVE_ACT_SIGMOID: return __fmul_rn(__fmul_rn(y, __fsub_rn(1.0f, y)), g);
-    case CLEAVE_ACT_RELU: return y > 0.0f ? g : 0.0f;
-    default: return g;
-  }
+template <int ACT>
+__device__ __forceinline__ float act_grad(float y, float g) {
+  if (ACT == CLEAVE_ACT_TANH) return __fmul_rn(__fsub_rn(1.0f, __fmul_rn(y, y)), g);
+  if (ACT == CLEAVE_ACT_SIGMOID) return __fmul_rn(__fmul_rn(y, __fsub_rn(1.0f, y)), g);
+  if (ACT == CLEAVE_ACT_RELU) return y > 0.0f ? g : 0.0f;
+  return g;
 }
 
-template <bool CHECKPOINT>
-__global__ void __launch_bounds__(kQThreads, 2) tile_kernel(const TileArgs a) {
-  __shared__ float s_max[kQWarps][kQBlock];
-  __shared__ float s_sum[CHECKPOINT ? kQWarps : 1][kQBlock];
-  __shared__ bool s_last;
+// What a tile's CTA shares: column maxima and column sums of each warp's rows, a word for the last-CTA test.
+struct TileShared {
+  float max[kQWarps][kQBlock];
+  float sum[kQWarps][kQBlock];
+  bool last;
+};
+
+constexpr int kNoAct = -1;   // plain quantization
+
+// One tile.  FULL: it lies inside the matrix and x can be read as 16-byte words, so that nothing is tested per row.
+template <int ACT, bool FULL>
+__device__ __forceinline__ void tile_pass(const TileArgs& a, TileShared& sh) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int col_blocks = (a.cols + kQBlock - 1) / kQBlock;
   const int rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
   const int r0 = rb * kQBlock + warp * kQRows, c0 = cb * kQBlock + lane * 4;
   const int64_t pitch = ((int64_t)a.cols + 15) / 16 * 16;
-  const int rows_here = a.rows - r0 < kQRows ? a.rows - r0 : kQRows;   // may be negative
+  const int rows_here = FULL ? kQRows : a.rows - r0 < kQRows ? a.rows - r0 : kQRows;   // may be negative
+  const bool in_pitch = FULL || c0 < pitch;   // the padding behind the last column gets zeros
 
   // ---- every load of the thread
   float v[kQRows][4];
   const float* src = a.x + (int64_t)r0 * a.cols + c0;
-  if (a.vec) {
+  if (FULL || a.vec) {
 #pragma unroll
     for (int i = 0; i < kQRows; ++i) {
       float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (i < rows_here && c0 < a.cols) t = __ldcs(reinterpret_cast<const float4*>(src + (int64_t)i * a.cols));
+      if (FULL || (i < rows_here && c0 < a.cols)) t = __ldcs(reinterpret_cast<const float4*>(src));
+      src += a.cols;
       v[i][0] = t.x; v[i][1] = t.y; v[i][2] = t.z; v[i][3] = t.w;
     }
   } else {
@@ -112,17 +121,19 @@ __global__ void __launch_bounds__(kQThreads, 2) tile_kernel(const TileArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[i][j] = i < rows_here && c0 + j < a.cols ? __ldg(src + (int64_t)i * a.cols + j) : 0.0f;
   }
-  if constexpr (CHECKPOINT) {
+  if constexpr (ACT != kNoAct) {
     uint32_t w[kQRows];
     const uint8_t* ysrc = a.y_q + r0 * pitch + c0;
 #pragma unroll
-    for (int i = 0; i < kQRows; ++i)
-      w[i] = i < rows_here && c0 < a.cols ? __ldcs(reinterpret_cast<const uint32_t*>(ysrc + i * pitch)) : 0u;
-    float sc[4];
+    for (int i = 0; i < kQRows; ++i) {
+      w[i] = FULL || (i < rows_here && c0 < a.cols) ? __ldcs(reinterpret_cast<const uint32_t*>(ysrc)) : 0u;
+      ysrc += pitch;
+    }
+    float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     float row_scale = 0.0f;   // ROWS: lane i holds row i's
     if (a.y_blocks == CLEAVE_BLOCKS_COLS) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sc[j] = c0 + j < a.cols ? __ldg(a.y_s + (int64_t)rb * a.cols + c0 + j) : 0.0f;
+      for (int j = 0; j < 4; ++j) sc[j] = FULL || c0 + j < a.cols ? __ldg(a.y_s + (int64_t)rb * a.cols + c0 + j) : 0.0f;
     } else if (a.y_blocks == CLEAVE_BLOCKS_TILES) {
       sc[0] = sc[1] = sc[2] = sc[3] = __ldg(a.y_s + (int64_t)rb * col_blocks + cb);
     } else {
@@ -134,16 +145,19 @@ __global__ void __launch_bounds__(kQThreads, 2) tile_kernel(const TileArgs a) {
       unpack4(w[i], y);
       if (a.y_blocks == CLEAVE_BLOCKS_ROWS) sc[0] = sc[1] = sc[2] = sc[3] = __shfl_sync(0xffffffffu, row_scale, i);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        v[i][j] = i < rows_here && c0 + j < a.cols ? act_grad(__fmul_rn(y[j], sc[j]), v[i][j], a.act) : 0.0f;   // padding bytes may be anything
+      for (int j = 0; j < 4; ++j) {
+        v[i][j] = act_grad<ACT>(__fmul_rn(y[j], sc[j]), v[i][j]);
+        if (!FULL && !(i < rows_here && c0 + j < a.cols)) v[i][j] = 0.0f;   // padding bytes may be anything
+      }
     }
     if (a.dz != nullptr) {
       float* dst = a.dz + (int64_t)r0 * a.cols + c0;
 #pragma unroll
       for (int i = 0; i < kQRows; ++i) {
-        if (i >= rows_here) break;
-        if (a.vec) {
-          if (c0 < a.cols) __stcs(reinterpret_cast<float4*>(dst + (int64_t)i * a.cols), make_float4(v[i][0], v[i][1], v[i][2], v[i][3]));
+        if (!FULL && i >= rows_here) break;
+        if (FULL || a.vec) {
+          if (FULL || c0 < a.cols)
+            __stcs(reinterpret_cast<float4*>(dst + (int64_t)i * a.cols), make_float4(v[i][0], v[i][1], v[i][2], v[i][3]));
         } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
@@ -157,107 +171,127 @@ __global__ void __launch_bounds__(kQThreads, 2) tile_kernel(const TileArgs a) {
       for (int i = 0; i < kQRows; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) sum[j] = __fadd_rn(sum[j], v[i][j]);
-      *reinterpret_cast<float4*>(&s_sum[warp][lane * 4]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+      *reinterpret_cast<float4*>(&sh.sum[warp][lane * 4]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
     }
   }
 #pragma unroll
   for (int i = 0; i < kQRows; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[i][j] = finite_or_nan(v[i][j]);
-  const bool in_pitch = c0 < pitch;   // the padding behind the last column gets zeros
 
   // ---- column maxima to shared memory
   const bool whole_tile = a.q_cols != nullptr || a.q_tiles != nullptr;
   if (whole_tile) {
-    float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m[4];
 #pragma unroll
-    for (int i = 0; i < kQRows; ++i)
+    for (int j = 0; j < 4; ++j) {
+      m[j] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], fabsf(v[i][j]));
-    *reinterpret_cast<float4*>(&s_max[warp][lane * 4]) = make_float4(m[0], m[1], m[2], m[3]);
+      for (int i = 0; i < kQRows; ++i) m[j] = fmaxf(m[j], fabsf(v[i][j]));
+    }
+    *reinterpret_cast<float4*>(&sh.max[warp][lane * 4]) = make_float4(m[0], m[1], m[2], m[3]);
   }
-  // ---- 1 x 128 blocks: a row of the tile is one warp's
+  // ---- 1 x 128 blocks: a row of the tile is one warp's.  Lane i works out row i's scale for all.
   if (a.q_rows != nullptr) {
-    float own_scale = 0.0f;
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < kQRows; ++i) {
+      // the leading 0 also replaces a NaN met first
+      const float m = fmaxf(fmaxf(fmaxf(0.0f, fabsf(v[i][0])), fabsf(v[i][1])), fmaxf(fmaxf(0.0f, fabsf(v[i][2])), fabsf(v[i][3])));
+      const uint32_t row_max = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+      mine = lane == i ? row_max : mine;
+    }
+    const uint32_t e = amax_exponent(mine);
+    if (lane < kQRows && lane < rows_here) a.s_rows[(int64_t)cb * a.rows + r0 + lane] = scale_of(e);
+    const float my_inv = inverse_scale_of(e);
     uint8_t* dst = a.q_rows + r0 * pitch + c0;
 #pragma unroll
     for (int i = 0; i < kQRows; ++i) {
-      const float m = fmaxf(fmaxf(fmaxf(0.0f, fabsf(v[i][0])), fabsf(v[i][1])), fmaxf(fmaxf(0.0f, fabsf(v[i][2])), fabsf(v[i][3])));
-      const uint32_t e = scale_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
-      if (lane == i) own_scale = scale_of(e);
-      const float inv = inverse_scale_of(e);
+      const float inv = __shfl_sync(0xffffffffu, my_inv, i);
       const float inv4[4] = {inv, inv, inv, inv};
-      if (i < rows_here && in_pitch) *reinterpret_cast<uint32_t*>(dst + i * pitch) = quantize4(v[i], inv4);
+      if (FULL || (i < rows_here && in_pitch)) *reinterpret_cast<uint32_t*>(dst) = quantize4(v[i], inv4);
+      dst += pitch;
     }
-    if (lane < rows_here && lane < kQRows) a.s_rows[(int64_t)cb * a.rows + r0 + lane] = own_scale;
   }
-  if (!whole_tile && (!CHECKPOINT || a.db_part == nullptr)) return;
+  const bool sums = ACT != kNoAct && a.db_part != nullptr;
+  if (!whole_tile && !sums) return;
   __syncthreads();
   if (whole_tile) {
     float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < kQWarps; ++w) {
-      const float4 t = *reinterpret_cast<const float4*>(&s_max[w][lane * 4]);
+      const float4 t = *reinterpret_cast<const float4*>(&sh.max[w][lane * 4]);
       m[0] = fmaxf(m[0], t.x); m[1] = fmaxf(m[1], t.y); m[2] = fmaxf(m[2], t.z); m[3] = fmaxf(m[3], t.w);
     }
     if (a.q_cols != nullptr) {
       float inv[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t e = scale_exponent(__float_as_uint(m[j]));
+        const uint32_t e = amax_exponent(__float_as_uint(m[j]));
         inv[j] = inverse_scale_of(e);
-        if (warp == 0 && c0 + j < a.cols) a.s_cols[(int64_t)rb * a.cols + c0 + j] = scale_of(e);
+        if (warp == 0 && (FULL || c0 + j < a.cols)) a.s_cols[(int64_t)rb * a.cols + c0 + j] = scale_of(e);
       }
       uint8_t* dst = a.q_cols + r0 * pitch + c0;
 #pragma unroll
-      for (int i = 0; i < kQRows; ++i)
-        if (i < rows_here && in_pitch) *reinterpret_cast<uint32_t*>(dst + i * pitch) = quantize4(v[i], inv);
+      for (int i = 0; i < kQRows; ++i) {
+        if (FULL || (i < rows_here && in_pitch)) *reinterpret_cast<uint32_t*>(dst) = quantize4(v[i], inv);
+        dst += pitch;
+      }
     }
     if (a.q_tiles != nullptr) {
-      const uint32_t e = scale_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])))));
+      const uint32_t e = amax_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])))));
       const float inv = inverse_scale_of(e);
       const float inv4[4] = {inv, inv, inv, inv};
       if (threadIdx.x == 0) a.s_tiles[(int64_t)rb * col_blocks + cb] = scale_of(e);
       uint8_t* dst = a.q_tiles + r0 * pitch + c0;
 #pragma unroll
-      for (int i = 0; i < kQRows; ++i)
-        if (i < rows_here && in_pitch) *reinterpret_cast<uint32_t*>(dst + i * pitch) = quantize4(v[i], inv4);
+      for (int i = 0; i < kQRows; ++i) {
+        if (FULL || (i < rows_here && in_pitch)) *reinterpret_cast<uint32_t*>(dst) = quantize4(v[i], inv4);
+        dst += pitch;
+      }
     }
   }
-  if constexpr (CHECKPOINT) {
+  if constexpr (ACT != kNoAct) {
     // ---- column sums: of the tile, then, by the last CTA of the column block to get here, of the row blocks in ascending
     // order, four runs of them side by side: the order of the additions is a function of the shape alone
-    if (a.db_part == nullptr) return;
+    if (!sums) return;
     const int tc = threadIdx.x & (kQBlock - 1), part = threadIdx.x / kQBlock;   // column, one of four
     const int c = cb * kQBlock + tc;
     if (part == 0 && c < a.cols) {
-      float t = s_sum[0][tc];
+      float t = sh.sum[0][tc];
 #pragma unroll
-      for (int w = 1; w < kQWarps; ++w) t = __fadd_rn(t, s_sum[w][tc]);
+      for (int w = 1; w < kQWarps; ++w) t = __fadd_rn(t, sh.sum[w][tc]);
       a.db_part[(int64_t)rb * a.cols + c] = t;
     }
     if (a.db == nullptr) return;
     const int row_blocks = (a.rows + kQBlock - 1) / kQBlock;
-    __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0) {   // releases what the CTA stored before the barrier, acquires what the others released
       unsigned int before;
       asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;"
                    : "=r"(before) : "l"(&g_db_arrivals[cb]), "r"((unsigned int)(row_blocks - 1)) : "memory");
-      s_last = before == (unsigned int)(row_blocks - 1);
+      sh.last = before == (unsigned int)(row_blocks - 1);
     }
     __syncthreads();
-    if (!s_last) return;
-    __threadfence();
+    if (!sh.last) return;
     const int per = (row_blocks + 3) / 4, first = part * per;
     float t = 0.0f;
     if (c < a.cols)
       for (int r = first; r < first + per && r < row_blocks; ++r) t = __fadd_rn(t, __ldcg(a.db_part + (int64_t)r * a.cols + c));
-    s_sum[part][tc] = t;
+    sh.sum[part][tc] = t;
     __syncthreads();
     if (part == 0 && c < a.cols)
-      a.db[c] = __fadd_rn(__fadd_rn(s_sum[0][tc], s_sum[1][tc]), __fadd_rn(s_sum[2][tc], s_sum[3][tc]));
+      a.db[c] = __fadd_rn(__fadd_rn(sh.sum[0][tc], sh.sum[1][tc]), __fadd_rn(sh.sum[2][tc], sh.sum[3][tc]));
   }
+}
+
+template <int ACT>
+__global__ void __launch_bounds__(kQThreads, 2) tile_kernel(const TileArgs a) {
+  __shared__ TileShared sh;
+  const int col_blocks = (a.cols + kQBlock - 1) / kQBlock;
+  const int rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
+  if (a.vec && rb < a.rows / kQBlock && cb < a.cols / kQBlock) tile_pass<ACT, true>(a, sh);
+  else tile_pass<ACT, false>(a, sh);
 }
 
 // out[r, c] = q * scale: one thread per four columns of a row.
@@ -347,10 +381,12 @@ static bool launch_tiles(const TileArgs& a, const char* what) {
     set_error(CLEAVE_CUDA_ERR_UNSUPPORTED, "%s: %d x %d has more than 2^31 - 1 blocks", what, a.rows, a.cols);
     return false;
   }
-  if (a.y_q)
-    tile_kernel<true><<<(int)tiles, kQThreads, 0, ctx().stream>>>(a);
-  else
-    tile_kernel<false><<<(int)tiles, kQThreads, 0, ctx().stream>>>(a);
+  cudaStream_t s = ctx().stream;
+  if (!a.y_q) tile_kernel<kNoAct><<<(int)tiles, kQThreads, 0, s>>>(a);
+  else if (a.act == CLEAVE_ACT_TANH) tile_kernel<CLEAVE_ACT_TANH><<<(int)tiles, kQThreads, 0, s>>>(a);
+  else if (a.act == CLEAVE_ACT_SIGMOID) tile_kernel<CLEAVE_ACT_SIGMOID><<<(int)tiles, kQThreads, 0, s>>>(a);
+  else if (a.act == CLEAVE_ACT_RELU) tile_kernel<CLEAVE_ACT_RELU><<<(int)tiles, kQThreads, 0, s>>>(a);
+  else tile_kernel<CLEAVE_ACT_IDENTITY><<<(int)tiles, kQThreads, 0, s>>>(a);
   count_launch();
   return cuda_ok(cudaGetLastError(), "quantize kernel launch");
 }
