@@ -97,9 +97,10 @@ __device__ __forceinline__ uint32_t cluster_size() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ float load_cluster_f32(uint32_t smem_addr, uint32_t rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(smem_addr, rank)) : "memory");
+__device__ __forceinline__ float4 load_cluster_f32x4(uint32_t smem_addr, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(map_to_cta(smem_addr, rank)));
   return v;
 }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
@@ -325,7 +326,9 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
   tcgen05_fence_after();
   const uint32_t tmem_base = tmem_slot;
   float* red = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)));   // the ring, once it is drained
-  constexpr int kRedPitch = BNQ + 1;
+  // Laid out as C is: along P for swapped sides, along Q otherwise, so that whole 16-byte words are read (from the other CTAs too,
+  // where 4-byte words at a stride cost 11 us of a 30 us product) and written; the pitches keep both free of bank conflicts.
+  constexpr int kRedPitch = BNQ + 4, kRedPitchSwap = 132;
 
   const int slots = p.stages + 3;
   if (warp == 0) {
@@ -429,42 +432,87 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
       if (++slot == slots) { slot = 0; slot_phase ^= 1u; }
     }
     // Every load has landed and every MMA has read it: the ring is free for the partial sums.
+    const int pr = quarter * 32 + lane;
+    if (p.swap) {
 #pragma unroll
-    for (int j = 0; j < T::kCols / 2; ++j) {
-      float* at = red + (quarter * 32 + lane) * kRedPitch + half * T::kCols + 2 * j;
-      at[0] = low_half(sum[j]);
-      at[1] = high_half(sum[j]);
+      for (int j = 0; j < T::kCols / 2; ++j) {
+        red[(half * T::kCols + 2 * j) * kRedPitchSwap + pr] = low_half(sum[j]);
+        red[(half * T::kCols + 2 * j + 1) * kRedPitchSwap + pr] = high_half(sum[j]);
+      }
+    } else {
+      float4* at = reinterpret_cast<float4*>(red + pr * kRedPitch + half * T::kCols);
+#pragma unroll
+      for (int j = 0; j < T::kCols / 4; ++j)
+        at[j] = make_float4(low_half(sum[2 * j]), high_half(sum[2 * j]), low_half(sum[2 * j + 1]), high_half(sum[2 * j + 1]));
     }
   }
 
   __syncwarp();
   tcgen05_fence_before();
   __syncthreads();
-  if (ranks > 1) cluster_sync_all();
-  if (!abort_flag) {
-    // This CTA's share of the tile's P rows, summed over the ranks in ascending order and stored along C's rows.
-    const int share = 128 / (int)ranks, first = (int)rank * share;
-    const int total = share * BNQ;
-    for (int i = threadIdx.x; i < total; i += T::kThreads) {
-      const int pr = first + (p.swap ? i % share : i / BNQ), qc = p.swap ? i / share : i % BNQ;
-      const int gp = pt * 128 + pr, gq = qt * BNQ + qc;
-      if (gp >= p.p_dim || gq >= p.q_dim) continue;
-      float v;
-      if (ranks == 1) {
-        v = red[pr * kRedPitch + qc];
+  // This CTA's share of the tile's P rows, four neighbours of C at a time, kBatch of those a thread: what does not depend on the
+  // sums (places, bias) is fetched before the barrier, and the CTA tells its peers that it has read theirs before it stores.
+  constexpr int kBatch = BNQ <= 64 ? 2 : 1;
+  const int share = 128 / (int)ranks, first = (int)rank * share;
+  const int inner4 = (p.swap ? share : BNQ) / 4, total = share * BNQ / 4;
+  const bool vec_ok = p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.c) & 15u) == 0;
+  bool arrived = false;
+  for (int base = 0; base < total; base += kBatch * T::kThreads) {   // the same trips for every thread
+    const float* at[kBatch];
+    int row[kBatch], col[kBatch];
+    float bias[kBatch][4];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = base + u * T::kThreads + (int)threadIdx.x;
+      const int outer = i / inner4, inner = (i - outer * inner4) * 4;
+      const int pr = first + (p.swap ? inner : outer), qc = p.swap ? outer : inner;
+      at[u] = p.swap ? red + qc * kRedPitchSwap + pr : red + pr * kRedPitch + qc;
+      row[u] = p.swap ? qt * BNQ + qc : pt * 128 + pr;
+      col[u] = p.swap ? pt * 128 + pr : qt * BNQ + qc;
+      if (i >= total) row[u] = p.m;   // nothing to do
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bias[u][e] = p.bias != nullptr && row[u] < p.m && col[u] + e < p.n ? __ldg(p.bias + col[u] + e) : 0.0f;
+    }
+    if (base == 0 && ranks > 1) cluster_sync_all();
+    float4 part[kBatch][kQMaxSplit];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+      for (int r = 0; r < kQMaxSplit; ++r)
+        if (row[u] < p.m && r < (int)ranks)
+          part[u][r] = ranks == 1 ? *reinterpret_cast<const float4*>(at[u]) : load_cluster_f32x4(smem_u32(at[u]), (uint32_t)r);
+    if (ranks > 1 && base + kBatch * T::kThreads >= total) {
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // the loads above have been performed
+      arrived = true;
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (row[u] >= p.m || col[u] >= p.n || abort_flag) continue;
+      float v[4] = {part[u][0].x, part[u][0].y, part[u][0].z, part[u][0].w};
+#pragma unroll
+      for (int r = 1; r < kQMaxSplit; ++r)   // in rank order
+        if (r < (int)ranks) {
+          v[0] = __fadd_rn(v[0], part[u][r].x);
+          v[1] = __fadd_rn(v[1], part[u][r].y);
+          v[2] = __fadd_rn(v[2], part[u][r].z);
+          v[3] = __fadd_rn(v[3], part[u][r].w);
+        }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = q_epilogue(p.bias != nullptr ? __fadd_rn(v[e], bias[u][e]) : v[e], p.act);
+      float* dst = p.c + (int64_t)row[u] * p.n + col[u];
+      if (vec_ok) {   // n and col are multiples of 4
+        *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
       } else {
-        const uint32_t at = smem_u32(red + pr * kRedPitch + qc);
-        v = load_cluster_f32(at, 0);
-        for (uint32_t r = 1; r < ranks; ++r) v = __fadd_rn(v, load_cluster_f32(at, r));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col[u] + e < p.n) dst[e] = v[e];
       }
-      const int row = p.swap ? gq : gp, col = p.swap ? gp : gq;
-      if (p.bias != nullptr) v = __fadd_rn(v, __ldg(p.bias + col));
-      p.c[(int64_t)row * p.n + col] = q_epilogue(v, p.act);
     }
   }
-  if (ranks > 1) {
+  if (arrived) {
     __syncwarp();
-    cluster_sync_all();   // the peers are done with this CTA's shared memory
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // the peers have read this CTA's shared memory
   }
   if (warp == 1) {
     tcgen05_fence_after();
