@@ -22,7 +22,7 @@ import numpy as np
 
 from . import nn
 from ._lib import lib, raise_last_error
-from .linalg import Tensor, dense_grads, gemm_into, split_lo
+from .linalg import QTensor, Tensor, dense_grads, gemm_into, gemm_q_into, quantize, split_lo
 
 _ACT_BWD = {"tanh": nn.tanh_bwd, "sigmoid": nn.sigmoid_bwd}
 
@@ -35,13 +35,20 @@ class MLP2:
     """
 
     def __init__(self, d_in: int, d_hid: int, d_out: int, act1: str = "tanh", act2: str = "sigmoid",
-                 params: Tensor | None = None, grads: Tensor | None = None, chain_lo: bool | None = None):
+                 params: Tensor | None = None, grads: Tensor | None = None, chain_lo: bool | None = None,
+                 products: str = "f32"):
         """``params`` / ``grads``: optional caller-provided flat buffers (e.g. views of symmetric
         memory shared with the other data-parallel ranks); allocated here when omitted.
         ``chain_lo``: hand the lo planes of the tensor-core split from one product to the next (each GEMM's
         epilogue writes the plane its consumer needs) instead of letting every product split its operands
         again; default: on for layer sizes that are multiples of 32 (what the tensor-core route needs to read
-        the tensors in place).  The gradients are bit-identical either way."""
+        the tensors in place).  The gradients are bit-identical either way.
+        ``products``: ``"f32"``, or ``"e4m3"`` for products of 8-bit operands with a scale per block of 128.  Parameters,
+        activations handed out, loss and gradients stay f32; between the forward and the backward pass the inputs of
+        both layers are kept in 8 bits only, a quarter of the memory, and the backward pass reads them as they are."""
+        if products not in ("f32", "e4m3"):
+            raise ValueError(f"products: 'f32' or 'e4m3', not {products!r}")
+        self.products = products
         if act1 not in _ACT_BWD or act2 not in _ACT_BWD:
             raise ValueError("activations with a declared derivative rule: tanh, sigmoid")
         self.d_in, self.d_hid, self.d_out, self.act1, self.act2 = d_in, d_hid, d_out, act1, act2
@@ -80,6 +87,12 @@ class MLP2:
 
     def forward(self, X: Tensor):
         batch = X.dims[0]
+        if self.products == "e4m3":
+            H = gemm_q_into(Tensor.empty(batch, self.d_hid), quantize(X, "rows"), quantize(self.W1, "tiles"), bias=self.b1,
+                            act=self.act1)
+            Y = gemm_q_into(Tensor.empty(batch, self.d_out), quantize(H, "rows"), quantize(self.W2, "tiles"), bias=self.b2,
+                            act=self.act2)
+            return H, Y
         H = gemm_into(Tensor.empty(batch, self.d_hid), X, self.W1, bias=self.b1, act=self.act1)
         Y = gemm_into(Tensor.empty(batch, self.d_out), H, self.W2, bias=self.b2, act=self.act2)
         return H, Y
@@ -96,6 +109,8 @@ class MLP2:
         may be ``None``); without them the step splits the weights itself when it chains planes.
         With ``loss_out`` (a one-element tensor) the loss is left on the device, nothing waits and
         ``None`` is returned."""
+        if self.products == "e4m3":
+            return self._forward_backward_e4m3(X, T, keep, on_grads_ready, loss_out, before_layer)
         if before_layer:
             before_layer(1)
         batch = X.dims[0]
@@ -146,9 +161,41 @@ class MLP2:
             return loss, dict(H=H, Y=Y, dZ2=dZ2, dH=dH, dZ1=dZ1)
         return loss
 
+    def _forward_backward_e4m3(self, X, T, keep, on_grads_ready, loss_out, before_layer):
+        """``forward_backward`` with 8-bit products.  Each tensor is quantized along the contraction of every product that
+        reads it -- rows for X W and dZ W^T, columns for X^T dZ -- from one read; weights in tiles serve both ways.  A
+        quantized value stands for the value itself in the backward pass (its rounding has no derivative)."""
+        if before_layer:
+            before_layer(1)
+        batch = X.dims[0]
+        X_rows, X_cols = quantize(X, "rows", "cols")
+        H = gemm_q_into(Tensor.empty(batch, self.d_hid), X_rows, quantize(self.W1, "tiles"), bias=self.b1, act=self.act1)
+        H_rows, H_cols = quantize(H, "rows", "cols")   # H_cols is all that the backward pass keeps of H
+        H = H if keep else None
+        if before_layer:
+            before_layer(2)
+        W2 = quantize(self.W2, "tiles")
+        Y = gemm_q_into(Tensor.empty(batch, self.d_out), H_rows, W2, bias=self.b2, act=self.act2)
+        loss, dZ2 = nn.mse_act_bwd(Y, T, self.act2, loss_out)
+        dZ2_rows, dZ2_cols = quantize(dZ2, "rows", "cols")
+        dH = gemm_q_into(Tensor.empty(batch, self.d_hid), dZ2_rows, W2, trans_b=True)
+        dZ1_cols = QTensor(batch, self.d_hid, "cols")
+        dZ1 = Tensor.empty(batch, self.d_hid) if keep else None
+        nn.act_bwd_q(H_cols, dH, self.act1, dZ1_cols, dz=dZ1, db=self.db1)
+        gemm_q_into(self.dW1, X_cols, dZ1_cols, trans_a=True)
+        if on_grads_ready:
+            on_grads_ready(1)
+        gemm_q_into(self.dW2, H_cols, dZ2_cols, trans_a=True)
+        nn.colsum_into(self.db2, dZ2)
+        if on_grads_ready:
+            on_grads_ready(0)
+        if keep:
+            return loss, dict(H=H, Y=Y, dZ2=dZ2, dH=dH, dZ1=dZ1)
+        return loss
+
     def chains_planes(self, batch: int) -> bool:
         """Whether a step at this batch size hands lo planes from product to product."""
-        return bool(self.chain_lo and batch % 32 == 0 and batch * self.d_in * self.d_hid >= (1 << 24))
+        return bool(self.products == "f32" and self.chain_lo and batch % 32 == 0 and batch * self.d_in * self.d_hid >= (1 << 24))
 
     def sgd(self, lr: float, gscale: float = 1.0) -> None:
         """``p = p - lr * gscale * g`` over the whole parameter buffer in one pass."""

@@ -267,13 +267,14 @@ class QTensor:
     row-major with a row pitch of ``cols`` rounded up to 16.  Scales are powers of two unless ``any_scales`` says otherwise.
     """
 
-    __slots__ = ("_h", "scales", "dims", "blocks", "any_scales")
+    __slots__ = ("_h", "scales", "dims", "blocks", "any_scales", "form")   # form: the block form as the C ABI spells it
 
     def __init__(self, rows: int, cols: int, blocks: str, *, any_scales: bool = False, _handle=None,
                  _scales: Tensor | None = None):
         """An uninitialised 8-bit tensor, the destination of ``quantize_into`` / ``nn.act_bwd_q``."""
         self._h = None
         self.dims, self.blocks, self.any_scales = _q_dims(rows, cols, blocks), blocks, bool(any_scales)
+        self.form = BLOCKS[blocks] | (SCALES_ANY if any_scales else 0)
         if _handle is None:
             _handle = lib().cleave_cuda_alloc_e4m3(self.nbytes)
             if not _handle:
@@ -312,11 +313,6 @@ class QTensor:
         if not h:
             raise_last_error("QTensor upload")
         return cls(*dims, blocks, any_scales=not powers, _handle=h, _scales=s)
-
-    @property
-    def form(self) -> int:
-        """The block form as the C ABI spells it."""
-        return BLOCKS[self.blocks] | (SCALES_ANY if self.any_scales else 0)
 
     @property
     def nbytes(self) -> int:
@@ -360,28 +356,24 @@ def _scale_dims(dims, blocks) -> tuple:
     return {"rows": (cb, rows), "cols": (rb, cols), "tiles": (rb, cb)}[blocks]
 
 
-def _q_outputs(what: str, dims, outs, forms) -> dict:
-    """``outs`` by block form; each at most once, each of shape ``dims``."""
-    got = {}
+def _q_outputs(what: str, dims, outs, forms: int) -> list:
+    """The handles of ``outs`` in the order of the C ABI, (bytes, scales) of rows, cols and, with three ``forms``, tiles; each
+    form at most once, each of shape ``dims``."""
+    handles = [None] * (2 * forms)
     for o in outs:
-        if not isinstance(o, QTensor) or o.blocks not in forms or o.blocks in got or o.dims != tuple(dims):
-            raise TypeError(f"{what}: cannot write {o!r}: want distinct forms out of {forms} of shape {tuple(dims)}")
-        got[o.blocks] = o
-    return got
-
-
-def _q_handles(got: dict, form: str) -> tuple:
-    o = got.get(form)
-    return (o._h, o.scales._h) if o is not None else (None, None)
+        at = 2 * BLOCKS[o.blocks] - 2 if isinstance(o, QTensor) else len(handles)
+        if at >= len(handles) or handles[at] is not None or o.dims != dims:
+            raise TypeError(f"{what}: cannot write {o!r}: want distinct forms out of {list(BLOCKS)[:forms]} of shape {dims}")
+        handles[at], handles[at + 1] = o._h, o.scales._h
+    return handles
 
 
 def quantize_into(x: Tensor, *outs: QTensor) -> None:
     """Quantizes ``x`` [rows, cols] into each of ``outs`` (one per block form) from one read of it."""
-    if len(x.dims) != 2 or x.dtype != "f32" or not outs:
+    dims = x.dims
+    if len(dims) != 2 or x.dtype != "f32" or not outs:
         raise TypeError(f"quantize: needs an f32 matrix and at least one output, got {x!r} and {len(outs)}")
-    got = _q_outputs("quantize", x.dims, outs, ("rows", "cols", "tiles"))
-    if lib().cleave_cuda_quantize_e4m3(x._h, *x.dims, *_q_handles(got, "rows"), *_q_handles(got, "cols"),
-                                       *_q_handles(got, "tiles")) != 0:
+    if lib().cleave_cuda_quantize_e4m3(x._h, *dims, *_q_outputs("quantize", dims, outs, 3)) != 0:
         raise_last_error("quantize")
 
 

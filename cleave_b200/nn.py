@@ -12,7 +12,7 @@ from __future__ import annotations
 import math
 
 from ._lib import lib, raise_last_error
-from .linalg import ACT, QTensor, Tensor, _q_handles, _q_outputs
+from .linalg import ACT, QTensor, Tensor, _q_outputs
 
 
 def _unary(what: str):
@@ -71,12 +71,11 @@ def act_bwd_q(y: QTensor, g: Tensor, act: str, *outs: QTensor, dz: Tensor | None
         raise TypeError(f"act_bwd_q: unknown activation {act!r}")
     if dz is not None and (dz.dims != y.dims or dz.dtype != "f32") or db is not None and (db.dims != y.dims[1:] or db.dtype != "f32"):
         raise TypeError(f"act_bwd_q: cannot write dz {dz!r}, db {db!r} for {y!r}")
-    got = _q_outputs("act_bwd_q", y.dims, outs, ("rows", "cols"))
-    if not got and dz is None and db is None:
+    if not outs and dz is None and db is None:
         raise TypeError("act_bwd_q: no output given")
-    h = lambda t: t._h if t is not None else None  # noqa: E731
-    if lib().cleave_cuda_act_bwd_e4m3(y._h, y.scales._h, y.form, g._h, *y.dims, ACT[act], h(dz),
-                                      *_q_handles(got, "rows"), *_q_handles(got, "cols"), h(db)) != 0:
+    h = _q_outputs("act_bwd_q", y.dims, outs, 2)
+    if lib().cleave_cuda_act_bwd_e4m3(y._h, y.scales._h, y.form, g._h, *y.dims, ACT[act], dz._h if dz is not None else None,
+                                      *h, db._h if db is not None else None) != 0:
         raise_last_error("act_bwd_q")
 
 
@@ -85,6 +84,14 @@ def colsum(x: Tensor) -> Tensor:
     if len(x.dims) != 2:
         raise TypeError("colsum needs a rank-2 tensor")
     return Tensor._wrap(lib().cleave_cuda_colsum_f32(x._h, x.dims[0], x.dims[1]), (x.dims[1],), "colsum")
+
+
+def colsum_into(out: Tensor, x: Tensor) -> None:
+    """``colsum`` written into ``out``."""
+    if len(x.dims) != 2 or out.dims != (x.dims[1],):
+        raise TypeError(f"colsum_into: {x!r} into {out!r}")
+    if lib().cleave_cuda_colsum_into_f32(out._h, x._h, x.dims[0], x.dims[1]) != 0:
+        raise_last_error("colsum_into")
 
 
 def bias_act(x: Tensor, bias: Tensor, act: str = "identity") -> Tensor:
