@@ -144,33 +144,11 @@ __device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
       : "memory");
 }
 
-// tanh(x) = x N(x^2) / D(x^2): a rational approximation of degree 4 / 4 (relative error 2.2e-8 on [-9.02, 9.02], fitted in
-// 50 digits for the least largest error; beyond, tanh rounds to 1), one reciprocal corrected to a division.  Within 3.4e-7 of
-// the value everywhere.  tanhf takes twice the instructions, and the epilogue of a product with a short contraction is
-// bound by them (4096 x 4096, k 1024: 48 us with it, 38 without an activation).
-__device__ __forceinline__ float q_tanh(float x) {
-  const float a = fabsf(x) > 9.02f ? copysignf(9.02f, x) : x;   // a NaN stays
-  const float s = __fmul_rn(a, a);
-  float n = 1.3328731e-8f, d = 7.7662906e-7f;
-  n = __fmaf_rn(n, s, 2.0591549e-5f);
-  d = __fmaf_rn(d, s, 3.2839418e-4f);
-  n = __fmaf_rn(n, s, 3.4945765e-3f);
-  d = __fmaf_rn(d, s, 2.5873192e-2f);
-  n = __fmaf_rn(n, s, 1.3380193e-1f);
-  d = __fmaf_rn(d, s, 4.6713510e-1f);
-  n = __fmul_rn(__fmaf_rn(n, s, 1.0f), a);
-  d = __fmaf_rn(d, s, 1.0f);
-  const float r = __fdividef(1.0f, d);
-  float q = __fmul_rn(n, r);
-  q = __fmaf_rn(__fmaf_rn(-q, d, n), r, q);
-  return fabsf(q) > 1.0f ? copysignf(1.0f, q) : q;
-}
-
 __device__ __forceinline__ float q_epilogue(float v, int act) {
   switch (act) {
     case CLEAVE_ACT_RELU: return act_apply(v, CLEAVE_ACT_RELU);
     case CLEAVE_ACT_SIGMOID: return __fdividef(1.0f, 1.0f + __expf(-v));   // as the f32 product's epilogue
-    case CLEAVE_ACT_TANH: return q_tanh(v);
+    case CLEAVE_ACT_TANH: return tanhf(v);
     default: return v;
   }
 }
@@ -583,27 +561,21 @@ __device__ __forceinline__ void copy_scales_pair(uint32_t tmem, uint32_t smem) {
   const uint64_t desc = make_smem_desc(smem, 128u, 0u, 0u);
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
-// Adds the bias, applies the activation and stores a drain warp's 32 x 32 block of C whose first element is (row0, col0);
+// Adds the bias (shared memory, 32 values), applies the activation and stores a drain warp's 32 x 32 block of C whose first element is (row0, col0);
 // lane r holds row r.  The block passes through the warp's staging tile (16-byte word j of row r at slot j ^ (r & 7):
 // conflict free both ways), so that every store instruction writes whole 128-byte lines.  Plain stores: bulk tensor stores of the
 // same tile queue in the copy engine before the next tile's loads, which then took 3000 to 4700 clocks to arrive.
-__device__ __forceinline__ void store_q_block(float (&v)[32], const TcParams& p, float4* stage, int row0, int col0, int lane,
-                                              bool vec_ok) {
+__device__ __forceinline__ void store_q_block(float (&v)[32], const TcParams& p, const float* bias, float4* stage, int row0,
+                                              int col0, int lane, bool vec_ok) {
   if (row0 >= p.m || col0 >= p.n) return;   // uniform over the warp
   if (p.bias != nullptr) {
-    if (col0 + 32 <= p.n && (reinterpret_cast<uintptr_t>(p.bias + col0) & 15u) == 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + col0) + j);
-        v[4 * j] = __fadd_rn(v[4 * j], b.x);
-        v[4 * j + 1] = __fadd_rn(v[4 * j + 1], b.y);
-        v[4 * j + 2] = __fadd_rn(v[4 * j + 2], b.z);
-        v[4 * j + 3] = __fadd_rn(v[4 * j + 3], b.w);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (col0 + j < p.n) v[j] = __fadd_rn(v[j], __ldg(p.bias + col0 + j));
+    for (int j = 0; j < 8; ++j) {
+      const float4 b = reinterpret_cast<const float4*>(bias)[j];
+      v[4 * j] = __fadd_rn(v[4 * j], b.x);
+      v[4 * j + 1] = __fadd_rn(v[4 * j + 1], b.y);
+      v[4 * j + 2] = __fadd_rn(v[4 * j + 2], b.z);
+      v[4 * j + 3] = __fadd_rn(v[4 * j + 3], b.w);
     }
   }
   if (p.act == CLEAVE_ACT_TANH) {
@@ -656,6 +628,7 @@ gemm_q_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
                    const QPairParams p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(128) uint8_t scale_words[kQScaleSlots][kQScaleSlotBytes];
+  __shared__ __align__(16) float bias_words[kQPairDrainWarps][kQPairCols];
   // full / done: a stage's bytes have landed (in CTA 0, for both) / its MMAs have read them; scale_full / scale_empty: the
   // same for a slot of scale words; acc_full / acc_empty: the accumulator is complete / has been read (in CTA 0)
   __shared__ __align__(8) uint64_t bar_full[kQPairStages];
@@ -873,13 +846,21 @@ gemm_q_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
     uint32_t acc_phase = 0;
     float4* stage_tile = reinterpret_cast<float4*>(smem_raw + (ring - smem_u32(smem_raw)) + kQPairRing + (warp - 4) * kQPairStaging);
     const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(part * kQPairCols);
+    float* bias_tile = bias_words[warp - 4];
     const bool vec_ok = p.t.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.t.c) & 15u) == 0;
     const uint32_t acc_empty0 = map_to_cta(smem_u32(&bar_acc_empty), 0);
     bool ok = true;
     for (int t = blockIdx.x >> 1; ok && t < tiles; t += n_clusters) {
       int mb, nb;
       decode_q_tile(t, p.t, mb, nb);
-      float sum[kQPairCols];
+      float sum[kQPairCols], bias[2] = {0.0f, 0.0f};   // the warp's 64 columns of the bias, two a lane, fetched long before their use
+      if (p.t.bias != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int col = nb * 256 + part * kQPairCols + i * 32 + lane;
+          if (col < p.t.n) bias[i] = __ldg(p.t.bias + col);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < kQPairCols; ++j) sum[j] = 0.0f;
       for (int kb = 0; kb < num_kb; kb += kQChunk) {
@@ -905,12 +886,16 @@ gemm_q_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
         acc_phase ^= 1u;
       }
       if (!ok) break;
+      __syncwarp();   // the last tile's have been read
+      bias_tile[lane] = bias[0];
+      bias_tile[lane + 32] = bias[1];
+      __syncwarp();
 #pragma unroll
       for (int pass = 0; pass < kQPairCols / 32; ++pass) {
         float v[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = sum[pass * 32 + j];
-        store_q_block(v, p.t, stage_tile, mb * 256 + (int)rank * 128 + quarter * 32, nb * 256 + part * kQPairCols + 32 * pass, lane,
+        store_q_block(v, p.t, bias_tile + 32 * pass, stage_tile, mb * 256 + (int)rank * 128 + quarter * 32, nb * 256 + part * kQPairCols + 32 * pass, lane,
                       vec_ok);
       }
     }
