@@ -17,6 +17,8 @@ f32 = np.float32
 FORMS = ["rows", "cols", "tiles"]
 SIZES = [(1, 1), (1, 128), (1, 1024), (3, 17), (128, 128), (129, 257), (200, 1000), (1000, 3), (257, 516), (130, 4100)]
 
+BIG = [(2300, 2100), (2177, 2511)]      # more tiles than are resident at once; 16-byte rows and others
+
 
 def wide(rows, cols, seed=0):
     """Values whose magnitudes differ from row to row and column to column by many powers of two, zeros among them."""
@@ -40,7 +42,7 @@ def at_offset(a: np.ndarray, floats: int) -> Tensor:
     return t
 
 
-@pytest.mark.parametrize("rows,cols", SIZES)
+@pytest.mark.parametrize("rows,cols", SIZES + BIG)
 def test_quantize_every_form_alone_and_together(rows, cols):
     x = wide(rows, cols)
     want = {f: qr.quantize(x, f) for f in FORMS}
@@ -143,7 +145,7 @@ def assert_colsum(got, dz):
     assert np.all(np.abs(got.astype(np.float64) - d64.sum(0)) <= bound)
 
 
-@pytest.mark.parametrize("rows,cols", SIZES)
+@pytest.mark.parametrize("rows,cols", SIZES + BIG)
 @pytest.mark.parametrize("act", ["tanh", "sigmoid", "relu", "identity"])
 def test_act_bwd_all_outputs(rows, cols, act):
     y, y_val = checkpoint(rows, cols, act, "cols")
