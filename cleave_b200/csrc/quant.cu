@@ -84,9 +84,11 @@ __device__ __forceinline__ float act_grad(float y, float g) {
   return g;
 }
 
-// What a tile's CTA shares: column maxima and column sums of each warp's rows, a word for the last-CTA test.
+// What a tile's CTA shares: the columns' maxima (bits of magnitudes, ordered as integers), the column sums of each warp's rows,
+// a word for the last-CTA test.  The maxima meet in shared-memory atomics: a maximum does not depend on the order, and every
+// warp reading the 16 warps' own ones took a sixth of the kernel's shared-memory cycles.
 struct TileShared {
-  float max[kQWarps][kQBlock];
+  uint32_t max[kQBlock];
   float sum[kQWarps][kQBlock];
   bool last;
 };
@@ -103,6 +105,9 @@ __device__ __forceinline__ void tile_pass(const TileArgs& a, TileShared& sh) {
   const int64_t pitch = ((int64_t)a.cols + 15) / 16 * 16;
   const int rows_here = FULL ? kQRows : a.rows - r0 < kQRows ? a.rows - r0 : kQRows;   // may be negative
   const bool in_pitch = FULL || c0 < pitch;   // the padding behind the last column gets zeros
+
+  const bool whole_tile = a.q_cols != nullptr || a.q_tiles != nullptr;
+  if (whole_tile && threadIdx.x < kQBlock) sh.max[threadIdx.x] = 0u;
 
   // ---- every load of the thread
   float v[kQRows][4];
@@ -180,8 +185,8 @@ __device__ __forceinline__ void tile_pass(const TileArgs& a, TileShared& sh) {
     for (int j = 0; j < 4; ++j) v[i][j] = finite_or_nan(v[i][j]);
 
   // ---- column maxima to shared memory
-  const bool whole_tile = a.q_cols != nullptr || a.q_tiles != nullptr;
   if (whole_tile) {
+    __syncthreads();   // they start at zero
     float m[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -189,7 +194,8 @@ __device__ __forceinline__ void tile_pass(const TileArgs& a, TileShared& sh) {
 #pragma unroll
       for (int i = 0; i < kQRows; ++i) m[j] = fmaxf(m[j], fabsf(v[i][j]));
     }
-    *reinterpret_cast<float4*>(&sh.max[warp][lane * 4]) = make_float4(m[0], m[1], m[2], m[3]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) atomicMax(&sh.max[lane * 4 + j], __float_as_uint(m[j]));
   }
   // ---- 1 x 128 blocks: a row of the tile is one warp's.  Lane i works out row i's scale for all.
   if (a.q_rows != nullptr) {
@@ -217,17 +223,13 @@ __device__ __forceinline__ void tile_pass(const TileArgs& a, TileShared& sh) {
   if (!whole_tile && !sums) return;
   __syncthreads();
   if (whole_tile) {
-    float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < kQWarps; ++w) {
-      const float4 t = *reinterpret_cast<const float4*>(&sh.max[w][lane * 4]);
-      m[0] = fmaxf(m[0], t.x); m[1] = fmaxf(m[1], t.y); m[2] = fmaxf(m[2], t.z); m[3] = fmaxf(m[3], t.w);
-    }
+    const uint4 m4 = *reinterpret_cast<const uint4*>(&sh.max[lane * 4]);
+    const uint32_t m[4] = {m4.x, m4.y, m4.z, m4.w};
     if (a.q_cols != nullptr) {
       float inv[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t e = amax_exponent(__float_as_uint(m[j]));
+        const uint32_t e = amax_exponent(m[j]);
         inv[j] = inverse_scale_of(e);
         if (warp == 0 && (FULL || c0 + j < a.cols)) a.s_cols[(int64_t)rb * a.cols + c0 + j] = scale_of(e);
       }
@@ -239,7 +241,7 @@ __device__ __forceinline__ void tile_pass(const TileArgs& a, TileShared& sh) {
       }
     }
     if (a.q_tiles != nullptr) {
-      const uint32_t e = amax_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])))));
+      const uint32_t e = amax_exponent(__reduce_max_sync(0xffffffffu, max(max(m[0], m[1]), max(m[2], m[3]))));
       const float inv = inverse_scale_of(e);
       const float inv4[4] = {inv, inv, inv, inv};
       if (threadIdx.x == 0) a.s_tiles[(int64_t)rb * col_blocks + cb] = scale_of(e);
@@ -287,7 +289,7 @@ __device__ __forceinline__ void tile_pass(const TileArgs& a, TileShared& sh) {
 
 template <int ACT>
 __global__ void __launch_bounds__(kQThreads, 2) tile_kernel(const TileArgs a) {
-  __shared__ TileShared sh;
+  __shared__ __align__(16) TileShared sh;
   const int col_blocks = (a.cols + kQBlock - 1) / kQBlock;
   const int rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
   if (a.vec && rb < a.rows / kQBlock && cb < a.cols / kQBlock) tile_pass<ACT, true>(a, sh);
