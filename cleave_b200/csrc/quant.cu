@@ -164,11 +164,19 @@ __device__ __forceinline__ void tile_pass(const TileArgs& a, TileShared& sh) {
           if (FULL || c0 < a.cols)
             __stcs(reinterpret_cast<float4*>(dst + (int64_t)i * a.cols), make_float4(v[i][0], v[i][1], v[i][2], v[i][3]));
         } else {
+          // rows that 16-byte words do not fit pass through the warp's shared row, so that a store covers whole lines: four
+          // 4-byte stores a stride of 16 bytes apart write every sector four times
+          float* row = sh.sum[warp];
+          __syncwarp();
+          *reinterpret_cast<float4*>(row + lane * 4) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+          __syncwarp();
+          float* out = a.dz + (int64_t)(r0 + i) * a.cols + cb * kQBlock + lane;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (c0 + j < a.cols) dst[(int64_t)i * a.cols + j] = v[i][j];
+            if (cb * kQBlock + lane + 32 * j < a.cols) __stcs(out + 32 * j, row[lane + 32 * j]);
         }
       }
+      __syncwarp();
     }
     if (a.db_part != nullptr) {
       float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
