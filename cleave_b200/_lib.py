@@ -7,6 +7,7 @@ library handle, and every compute call fails loudly when no CUDA device is prese
 from __future__ import annotations
 
 import ctypes
+import operator
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -18,6 +19,15 @@ c_f64p = ctypes.POINTER(ctypes.c_double)
 c_u8p = ctypes.POINTER(ctypes.c_uint8)
 f64 = ctypes.c_double
 i32, i64, f32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+
+
+
+class _Int32:
+    """Converts an ``int32_t`` argument.  ``operator.index`` refuses what is no integer, as ``c_int32`` does, but makes no object of
+    it: an 8-bit product's call, eight of whose fourteen arguments are such, takes 1.3 us instead of 4.4."""
+
+    from_param = operator.index
+
 
 # name -> (restype, argtypes); mirrors include/cleave_cuda.h declaration by declaration.
 SIGNATURES = {
@@ -164,7 +174,7 @@ def lib() -> ctypes.CDLL:
         for name, (res, args) in SIGNATURES.items():
             fn = getattr(L, name)
             fn.restype = res
-            fn.argtypes = args
+            fn.argtypes = [_Int32 if a is i32 else a for a in args]
         _lib = L
     return _lib
 
