@@ -105,7 +105,7 @@ __device__ __forceinline__ void finish_sums(const TileArgs& a, TileShared& sh, i
     a.db_part[(int64_t)rb * a.cols + c] = t;
   }
   if (a.db == nullptr) return;
-  const int row_blocks = (a.rows + kQBlock - 1) / kQBlock;
+  const int row_blocks = q_blocks(a.rows);
   __syncthreads();
   if (threadIdx.x == 0) {   // releases what the CTA stored before the barrier, acquires what the others released
     unsigned int before;
@@ -131,7 +131,7 @@ constexpr int kNoAct = -1;   // plain quantization
 template <int ACT, bool FULL>
 __device__ __forceinline__ void tile_pass(const TileArgs& a, TileShared& sh) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int col_blocks = (a.cols + kQBlock - 1) / kQBlock;
+  const int col_blocks = q_blocks(a.cols);
   const int rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
   const int r0 = rb * kQBlock + warp * kQRows, c0 = cb * kQBlock + lane * 4;
   const int64_t pitch = ((int64_t)a.cols + 15) / 16 * 16;
@@ -303,7 +303,7 @@ template <int ACT>
 __global__ void __launch_bounds__(kQThreads, 2) act_bwd_kernel(const TileArgs a) {
   __shared__ __align__(16) TileShared sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int col_blocks = (a.cols + kQBlock - 1) / kQBlock;
+  const int col_blocks = q_blocks(a.cols);
   const int rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
   const int r0 = rb * kQBlock + warp * kQRows, c0 = cb * kQBlock + lane;
   const int64_t pitch = ((int64_t)a.cols + 15) / 16 * 16;
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kQThreads, 2) act_bwd_kernel(const TileArgs a)
 template <int ACT>
 __global__ void __launch_bounds__(kQThreads, 2) tile_kernel(const TileArgs a) {
   __shared__ __align__(16) TileShared sh;
-  const int col_blocks = (a.cols + kQBlock - 1) / kQBlock;
+  const int col_blocks = q_blocks(a.cols);
   const int rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
   if (a.vec && rb < a.rows / kQBlock && cb < a.cols / kQBlock) tile_pass<ACT, true>(a, sh);
   else tile_pass<ACT, false>(a, sh);
@@ -366,8 +366,8 @@ __global__ void __launch_bounds__(kQThreads, 2) tile_kernel(const TileArgs a) {
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ q, const float* __restrict__ s,
                                                          float* __restrict__ out, int rows, int cols, int blocks, int vec) {
   const int64_t pitch = ((int64_t)cols + 15) / 16 * 16;
-  const int col_blocks = (cols + kQBlock - 1) / kQBlock;
-  const int groups = (cols + 3) / 4;
+  const int col_blocks = q_blocks(cols);
+  const int groups = (cols - 1) / 4 + 1;
   const int64_t total = (int64_t)rows * groups;
   for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < total; t += (int64_t)gridDim.x * blockDim.x) {
     const int r = (int)(t / groups), c = (int)(t - (int64_t)r * groups) * 4;
@@ -450,7 +450,7 @@ static void launch_act_bwd(const TileArgs& a, int tiles) {
 }
 
 static bool launch_tiles(const TileArgs& a, const char* what) {
-  const int64_t tiles = (((int64_t)a.rows + kQBlock - 1) / kQBlock) * (((int64_t)a.cols + kQBlock - 1) / kQBlock);
+  const int64_t tiles = (int64_t)q_blocks(a.rows) * q_blocks(a.cols);
   if (tiles > 0x7fffffffll) {
     set_error(CLEAVE_CUDA_ERR_UNSUPPORTED, "%s: %d x %d has more than 2^31 - 1 blocks", what, a.rows, a.cols);
     return false;
@@ -567,7 +567,7 @@ int32_t cleave_cuda_dequantize_e4m3(cleave_buf out, cleave_buf q, cleave_buf s, 
   const MemRange ins[2] = {{in.q, q_bytes(rows, cols)}, {in.s, q_scales(rows, cols, blocks) * 4}};
   if (!ranges_distinct(outs, 1, ins, 2, "dequantize")) return -cleave_cuda_last_error();
   Trace tr("dequantize", "rows=%d cols=%d blocks=%d", rows, cols, blocks);
-  dequantize_kernel<<<stream_grid((int64_t)rows * ((cols + 3) / 4), 256, 8), 256, 0, ctx().stream>>>(
+  dequantize_kernel<<<stream_grid((int64_t)rows * ((cols - 1) / 4 + 1), 256, 8), 256, 0, ctx().stream>>>(
       in.q, in.s, O->ptr, rows, cols, blocks, aligned16(O->ptr) && cols % 4 == 0);
   count_launch();
   return cuda_ok(cudaGetLastError(), "dequantize kernel launch") ? CLEAVE_CUDA_OK : -cleave_cuda_last_error();
@@ -632,8 +632,8 @@ int32_t cleave_cuda_act_bwd_e4m3(cleave_buf y, cleave_buf y_scale, int32_t y_blo
   a.q_cols = o[1].q; a.s_cols = o[1].s;
   // Column sums: every tile leaves the sums of its 128 rows; the kernel adds the row blocks itself, or, where there are more
   // column blocks than counters, a second one does.
-  const int row_blocks = ceil_div(rows, kQBlock);
-  const bool in_kernel = ceil_div(cols, kQBlock) <= kQMaxColBlocks;
+  const int row_blocks = q_blocks(rows);
+  const bool in_kernel = q_blocks(cols) <= kQMaxColBlocks;
   float* part = nullptr;
   if (DB) {
     part = row_blocks == 1 ? DB->ptr : scratch_alloc((int64_t)row_blocks * cols * (int64_t)sizeof(float));

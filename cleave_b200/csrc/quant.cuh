@@ -16,10 +16,12 @@ namespace cleave {
 
 constexpr int kQBlock = 128;
 
+// Blocks along a side of n >= 1 elements; n + 127 would pass 2^31 for the longest sides.
+__host__ __device__ constexpr int q_blocks(int n) { return (n - 1) / kQBlock + 1; }
 inline int64_t q_pitch(int cols) { return ((int64_t)cols + 15) / 16 * 16; }
 inline int64_t q_bytes(int rows, int cols) { return (int64_t)rows * q_pitch(cols); }
 inline int64_t q_scales(int rows, int cols, int blocks) {
-  const int64_t rb = ((int64_t)rows + kQBlock - 1) / kQBlock, cb = ((int64_t)cols + kQBlock - 1) / kQBlock;
+  const int64_t rb = q_blocks(rows), cb = q_blocks(cols);
   switch (blocks) {
     case CLEAVE_BLOCKS_ROWS: return cb * rows;
     case CLEAVE_BLOCKS_COLS: return rb * cols;
