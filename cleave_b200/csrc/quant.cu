@@ -24,7 +24,11 @@ namespace cleave {
 constexpr int kQThreads = 512;
 constexpr int kQWarps = kQThreads / 32;
 constexpr int kQRows = kQBlock / kQWarps;   // rows of the tile per warp
-constexpr int kQMaxColBlocks = 4096;        // column sums finished in the kernel up to this many
+// Column sums are finished in the kernel up to so many column blocks (counters) and row blocks (the last CTA's walk over them),
+// beyond that by colsum_launch.  In the kernel / by a second one, us: 128 row blocks (16384 x 1024) 28.7 / 29.3, 256 49.5 / 47.4, 512
+// 99.7 / 88.4, 8192 (1048576 x 128) 398 / 161.
+constexpr int kQMaxColBlocks = 4096;
+constexpr int kQMaxRowBlocks = 128;
 
 struct TileArgs {
   int rows, cols;
@@ -297,8 +301,9 @@ __device__ __forceinline__ void tile_pass(const TileArgs& a, TileShared& sh) {
 }
 
 // f32 output and column sums only: nothing has to be neighbours for packing, so a lane's columns are 32 apart and every load and
-// store of a warp covers whole lines whatever the alignment, four rows of a warp in flight at a time.  (6007 x 1283: 28.7 us
-// with tile_pass, whose 4-byte loads 16 bytes apart keep L1 70 % busy.)
+// store of a warp covers whole lines whatever the alignment, four rows of a warp in flight at a time.  For rows that 16-byte
+// words do not fit: 6007 x 1283 26.7 us, 28.7 with tile_pass, whose 4-byte loads 16 bytes apart keep L1 70 % busy; where they fit,
+// tile_pass is the faster (4096 x 4096: 27.8 us against 39.7).
 template <int ACT>
 __global__ void __launch_bounds__(kQThreads, 2) act_bwd_kernel(const TileArgs a) {
   __shared__ __align__(16) TileShared sh;
@@ -445,7 +450,7 @@ bool ranges_distinct(const MemRange* out, int n_out, const MemRange* in, int n_i
 
 template <int ACT>
 static void launch_act_bwd(const TileArgs& a, int tiles) {
-  if (a.q_rows || a.q_cols) tile_kernel<ACT><<<tiles, kQThreads, 0, ctx().stream>>>(a);
+  if (a.q_rows || a.q_cols || a.vec) tile_kernel<ACT><<<tiles, kQThreads, 0, ctx().stream>>>(a);
   else act_bwd_kernel<ACT><<<tiles, kQThreads, 0, ctx().stream>>>(a);
 }
 
@@ -630,10 +635,9 @@ int32_t cleave_cuda_act_bwd_e4m3(cleave_buf y, cleave_buf y_scale, int32_t y_blo
   a.dz = DZ ? DZ->ptr : nullptr;
   a.q_rows = o[0].q; a.s_rows = o[0].s;
   a.q_cols = o[1].q; a.s_cols = o[1].s;
-  // Column sums: every tile leaves the sums of its 128 rows; the kernel adds the row blocks itself, or, where there are more
-  // column blocks than counters, a second one does.
+  // Column sums: every tile leaves the sums of its 128 rows; the kernel adds the row blocks itself, or a second one does.
   const int row_blocks = q_blocks(rows);
-  const bool in_kernel = q_blocks(cols) <= kQMaxColBlocks;
+  const bool in_kernel = q_blocks(cols) <= kQMaxColBlocks && row_blocks <= kQMaxRowBlocks;
   float* part = nullptr;
   if (DB) {
     part = row_blocks == 1 ? DB->ptr : scratch_alloc((int64_t)row_blocks * cols * (int64_t)sizeof(float));
