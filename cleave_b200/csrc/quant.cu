@@ -25,13 +25,15 @@ constexpr int kQThreads = 512;
 constexpr int kQWarps = kQThreads / 32;
 constexpr int kQRows = kQBlock / kQWarps;   // rows of the tile per warp
 // Column sums are finished in the kernel up to so many column blocks (counters) and row blocks (the last CTA's walk over them),
-// beyond that by colsum_launch.  In the kernel / by a second one, us: 128 row blocks (16384 x 1024) 28.7 / 29.3, 256 49.5 / 47.4, 512
-// 99.7 / 88.4, 8192 (1048576 x 128) 398 / 161.
+// beyond that by colsum_launch.  In the kernel / by a second one, us: 128 row blocks (16384 x 1024) 28.7 / 29.3, 256 49.5 / 47.4,
+// 512 99.7 / 88.4, 8192 (1048576 x 128) 398 / 161.
 constexpr int kQMaxColBlocks = 4096;
 constexpr int kQMaxRowBlocks = 128;
 
 struct TileArgs {
   int rows, cols;
+  int row_blocks, col_blocks;   // q_blocks of them: tile_kernel, short of registers, spills less when it need not work them out
+                                // (4096 x 4096, tanh, two forms and sums: 28.7 us against 34.6)
   int vec;                // x (and dz) are 16-byte aligned and cols is a multiple of 4
   const float* x;         // [rows, cols]: the values, or the upstream gradient
   const uint8_t* y_q;     // checkpoint of the activation's output (null: plain quantization)
@@ -99,7 +101,7 @@ struct TileShared {
 
 // Column sums of a tile from its warps' (sh.sum, complete for the CTA), then, by the last CTA of the column block to get here, of
 // the row blocks in ascending order, four runs of them side by side: the order of the additions is a function of the shape alone.
-__device__ __forceinline__ void finish_sums(const TileArgs& a, TileShared& sh, int rb, int cb) {
+__device__ __forceinline__ void finish_sums(const TileArgs& a, TileShared& sh, int rb, int cb, int row_blocks) {
   const int tc = threadIdx.x & (kQBlock - 1), part = threadIdx.x / kQBlock;   // column, one of four
   const int c = cb * kQBlock + tc;
   if (part == 0 && c < a.cols) {
@@ -109,7 +111,6 @@ __device__ __forceinline__ void finish_sums(const TileArgs& a, TileShared& sh, i
     a.db_part[(int64_t)rb * a.cols + c] = t;
   }
   if (a.db == nullptr) return;
-  const int row_blocks = q_blocks(a.rows);
   __syncthreads();
   if (threadIdx.x == 0) {   // releases what the CTA stored before the barrier, acquires what the others released
     unsigned int before;
@@ -135,7 +136,7 @@ constexpr int kNoAct = -1;   // plain quantization
 template <int ACT, bool FULL>
 __device__ __forceinline__ void tile_pass(const TileArgs& a, TileShared& sh) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int col_blocks = q_blocks(a.cols);
+  const int col_blocks = a.col_blocks;
   const int rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
   const int r0 = rb * kQBlock + warp * kQRows, c0 = cb * kQBlock + lane * 4;
   const int64_t pitch = ((int64_t)a.cols + 15) / 16 * 16;
@@ -297,12 +298,12 @@ __device__ __forceinline__ void tile_pass(const TileArgs& a, TileShared& sh) {
       }
     }
   }
-  if (sums) finish_sums(a, sh, rb, cb);
+  if (sums) finish_sums(a, sh, rb, cb, a.row_blocks);
 }
 
 // f32 output and column sums only: nothing has to be neighbours for packing, so a lane's columns are 32 apart and every load and
 // store of a warp covers whole lines whatever the alignment, four rows of a warp in flight at a time.  For rows that 16-byte
-// words do not fit: 6007 x 1283 26.7 us, 28.7 with tile_pass, whose 4-byte loads 16 bytes apart keep L1 70 % busy; where they fit,
+// words do not fit: 6007 x 1283 24.6 us, 28.7 with tile_pass, whose 4-byte loads 16 bytes apart keep L1 70 % busy; where they fit,
 // tile_pass is the faster (4096 x 4096: 27.8 us against 39.7).
 template <int ACT>
 __global__ void __launch_bounds__(kQThreads, 2) act_bwd_kernel(const TileArgs a) {
@@ -355,13 +356,13 @@ __global__ void __launch_bounds__(kQThreads, 2) act_bwd_kernel(const TileArgs a)
 #pragma unroll
   for (int j = 0; j < 4; ++j) sh.sum[warp][lane + 32 * j] = sum[j];
   __syncthreads();
-  finish_sums(a, sh, rb, cb);
+  finish_sums(a, sh, rb, cb, q_blocks(a.rows));
 }
 
 template <int ACT>
 __global__ void __launch_bounds__(kQThreads, 2) tile_kernel(const TileArgs a) {
   __shared__ __align__(16) TileShared sh;
-  const int col_blocks = q_blocks(a.cols);
+  const int col_blocks = a.col_blocks;
   const int rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
   if (a.vec && rb < a.rows / kQBlock && cb < a.cols / kQBlock) tile_pass<ACT, true>(a, sh);
   else tile_pass<ACT, false>(a, sh);
@@ -455,7 +456,7 @@ static void launch_act_bwd(const TileArgs& a, int tiles) {
 }
 
 static bool launch_tiles(const TileArgs& a, const char* what) {
-  const int64_t tiles = (int64_t)q_blocks(a.rows) * q_blocks(a.cols);
+  const int64_t tiles = (int64_t)a.row_blocks * a.col_blocks;
   if (tiles > 0x7fffffffll) {
     set_error(CLEAVE_CUDA_ERR_UNSUPPORTED, "%s: %d x %d has more than 2^31 - 1 blocks", what, a.rows, a.cols);
     return false;
@@ -550,6 +551,8 @@ int32_t cleave_cuda_quantize_e4m3(cleave_buf x, int32_t rows, int32_t cols, clea
   TileArgs a{};
   a.rows = rows;
   a.cols = cols;
+  a.row_blocks = q_blocks(rows);
+  a.col_blocks = q_blocks(cols);
   a.vec = aligned16(X->ptr) && cols % 4 == 0;
   a.x = X->ptr;
   a.q_rows = o[0].q; a.s_rows = o[0].s;
@@ -626,6 +629,8 @@ int32_t cleave_cuda_act_bwd_e4m3(cleave_buf y, cleave_buf y_scale, int32_t y_blo
   TileArgs a{};
   a.rows = rows;
   a.cols = cols;
+  a.row_blocks = q_blocks(rows);
+  a.col_blocks = q_blocks(cols);
   a.vec = aligned16(G->ptr) && (!DZ || aligned16(DZ->ptr)) && cols % 4 == 0;
   a.x = G->ptr;
   a.y_q = Y.q;
