@@ -217,12 +217,16 @@ __device__ __forceinline__ void tmem_ld_wait_piece(uint32_t taddr, uint32_t (&r)
     tmem_wait_16(r);
   }
 }
-template <int COLS, int PIECE, bool QVEC, class Release>
-__device__ __forceinline__ void drain_columns(uint64_t (&sum)[COLS / 2], uint32_t taddr, float scale_p, const float* scale_q,
-                                              Release release) {
+// Neither the scales' product nor one scale's with the block's sum may leave the range of f32 where the result does not (scales of 2^70
+// and 2^60 for a sum of 2^-12).  A block's sum is 0 or from 2^-18 to 2^25, so its product with one scale is safe while that scale is
+// within 2^-100 and 2^100, and the scales may be multiplied first while that product is a normal number.  Beyond that, the row's scale is
+// brought back by a power of two that is multiplied on last: sum * scale_p' * scale_q, then sum += that * back.  A scale above 2^100
+// is lowered by 2^32 only, so that the smallest scale of the other side does not lose bits; where a step overflows, the result does.
+template <int COLS, int PIECE, bool QVEC, bool BEYOND, class Release>
+__device__ __forceinline__ void drain_pieces(uint64_t (&sum)[COLS / 2], uint32_t taddr, float one, float back, const float* scale_q,
+                                             Release release) {
   constexpr int kPiece = PIECE;
-  const float both = QVEC ? scale_p : __fmul_rn(scale_p, *scale_q);
-  const uint64_t both2 = pack2(__float_as_uint(both), __float_as_uint(both));
+  const uint64_t one2 = pack2(__float_as_uint(one), __float_as_uint(one)), back2 = pack2(__float_as_uint(back), __float_as_uint(back));
 #pragma unroll
   for (int g = 0; g < COLS / kPiece; ++g) {
     uint32_t r[kPiece];
@@ -232,15 +236,32 @@ __device__ __forceinline__ void drain_columns(uint64_t (&sum)[COLS / 2], uint32_
     for (int j = 0; j < kPiece / 2; j += 2) {
       const uint64_t v0 = pack2(r[2 * j], r[2 * j + 1]), v1 = pack2(r[2 * j + 2], r[2 * j + 3]);
       uint64_t &s0 = sum[g * kPiece / 2 + j], &s1 = sum[g * kPiece / 2 + j + 1];
-      if constexpr (QVEC) {
-        const ulonglong2 q = reinterpret_cast<const ulonglong2*>(scale_q)[g * kPiece / 4 + j / 2];
-        s0 = fma2(mul2(v0, both2), q.x, s0);
-        s1 = fma2(mul2(v1, both2), q.y, s1);
+      ulonglong2 q;
+      if constexpr (QVEC) q = reinterpret_cast<const ulonglong2*>(scale_q)[g * kPiece / 4 + j / 2];
+      else if constexpr (BEYOND) q.x = q.y = pack2(__float_as_uint(*scale_q), __float_as_uint(*scale_q));
+      if constexpr (BEYOND) {
+        s0 = fma2(mul2(mul2(v0, one2), q.x), back2, s0);
+        s1 = fma2(mul2(mul2(v1, one2), q.y), back2, s1);
+      } else if constexpr (QVEC) {
+        s0 = fma2(mul2(v0, one2), q.x, s0);
+        s1 = fma2(mul2(v1, one2), q.y, s1);
       } else {
-        s0 = fma2(v0, both2, s0);
-        s1 = fma2(v1, both2, s1);
+        s0 = fma2(v0, one2, s0);
+        s1 = fma2(v1, one2, s1);
       }
     }
+  }
+}
+template <int COLS, int PIECE, bool QVEC, class Release>
+__device__ __forceinline__ void drain_columns(uint64_t (&sum)[COLS / 2], uint32_t taddr, float scale_p, const float* scale_q,
+                                              Release release) {
+  const float both = QVEC ? scale_p : __fmul_rn(scale_p, *scale_q);
+  constexpr float kMost = QVEC ? 0x1p100f : 0x1.fffffep127f, kLeast = QVEC ? 0x1p-100f : 0x1p-126f;
+  if (__all_sync(0xffffffffu, fabsf(both) >= kLeast && fabsf(both) <= kMost)) {
+    drain_pieces<COLS, PIECE, QVEC, false>(sum, taddr, both, 1.0f, scale_q, release);
+  } else {
+    const float a = fabsf(scale_p), by = a > 0x1p100f ? 0x1p-32f : a < 0x1p-100f ? 0x1p64f : 1.0f;
+    drain_pieces<COLS, PIECE, QVEC, true>(sum, taddr, __fmul_rn(scale_p, by), __frcp_rn(by), scale_q, release);
   }
 }
 __device__ __forceinline__ float low_half(uint64_t v) { return __uint_as_float((uint32_t)v); }
@@ -400,7 +421,9 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
       }
       tcgen05_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BNQ + half * T::kCols);
-      drain_columns<T::kCols, T::kCols < 32 ? T::kCols : 32, QVEC>(sum, taddr, scale_p[slot][quarter * 32 + lane], &scale_q[slot][QVEC ? half * T::kCols : 0], [&] {
+      // 64 columns a warp leave no registers for pieces of 32: they spill (4096 x 4096 x k1024 of any scales 94 us against 78)
+      drain_columns<T::kCols, T::kCols == 32 ? 32 : 16, QVEC>(sum, taddr, scale_p[slot][quarter * 32 + lane],
+                                                              &scale_q[slot][QVEC ? half * T::kCols : 0], [&] {
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_tmem_empty[acc]));

@@ -385,7 +385,7 @@ int32_t cleave_cuda_quantize_e4m3(cleave_buf x, int32_t rows, int32_t cols, clea
                                   cleave_buf q_cols, cleave_buf s_cols, cleave_buf q_tiles, cleave_buf s_tiles);
 /* out[rows, cols] = byte * scale, rounded once (exact when the scale is a power of two). */
 int32_t cleave_cuda_dequantize_e4m3(cleave_buf out, cleave_buf q, cleave_buf s, int32_t rows, int32_t cols, int32_t blocks);
-/* c[m, n] = act(op(A) * op(B) + bias), all sums in f32.  Stored layouts as in cleave_cuda_gemm_ex_f32: A [m,k] ([k,m] if
+/* c[m, n] = act(op(A) * op(B) + bias), all sums in f32; a result that fits f32 is not lost to scales whose product does not.  Stored layouts as in cleave_cuda_gemm_ex_f32: A [m,k] ([k,m] if
  * trans_a), B [k,n] ([n,k] if trans_b).  Blocks run along the contraction or are tiles: A ROWS (COLS if trans_a) or TILES,
  * B COLS (ROWS if trans_b) or TILES, each plus CLEAVE_SCALES_ANY where its scales are not powers of two.  bias may be NULL (n elements otherwise).  Any
  * size from 1 up.  A layer's products: X W (X ROWS, W TILES), dZ W^T (dZ ROWS, W TILES, trans_b), X^T dZ (both COLS,
