@@ -162,6 +162,22 @@ __device__ __forceinline__ float q_epilogue(float v, int act) {
   }
 }
 
+// One choice for all of a thread's values: choosing for each of them spreads the code over more instruction lines, which a launch of
+// one k-block fetches cold.
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], int act) {
+  if (act == CLEAVE_ACT_TANH) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = q_epilogue(v[j], CLEAVE_ACT_TANH);
+  } else if (act == CLEAVE_ACT_SIGMOID) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = q_epilogue(v[j], CLEAVE_ACT_SIGMOID);
+  } else if (act == CLEAVE_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = q_epilogue(v[j], CLEAVE_ACT_RELU);
+  }
+}
+
 // Arrival on a barrier of another CTA without the release of this thread's earlier writes: what it announces is that TMEM
 // loads have completed (tcgen05.wait::ld), there is no memory to publish.  The releasing form waits for the warp's
 // outstanding traffic, 1000 to 1300 clocks here, twice what a k-block's MMAs take (8192^3: 1.02 ms against 0.6).
@@ -509,7 +525,8 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
           v[3] = __fadd_rn(v[3], part[u][r].w);
         }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = q_epilogue(p.bias != nullptr ? __fadd_rn(v[e], bias[u][e]) : v[e], p.act);
+      for (int e = 0; e < 4; ++e) v[e] = p.bias != nullptr ? __fadd_rn(v[e], bias[u][e]) : v[e];
+      activate(v, p.act);
       float* dst = p.c + (int64_t)row[u] * p.n + col[u];
       if (vec_ok) {   // n and col are multiples of 4
         *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
@@ -612,16 +629,7 @@ __device__ __forceinline__ void store_q_block(float (&v)[32], const TcParams& p,
       v[4 * j + 3] = __fadd_rn(v[4 * j + 3], b.w);
     }
   }
-  if (p.act == CLEAVE_ACT_TANH) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = q_epilogue(v[j], CLEAVE_ACT_TANH);
-  } else if (p.act == CLEAVE_ACT_SIGMOID) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = q_epilogue(v[j], CLEAVE_ACT_SIGMOID);
-  } else if (p.act == CLEAVE_ACT_RELU) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = q_epilogue(v[j], CLEAVE_ACT_RELU);
-  }
+  activate(v, p.act);
   __syncwarp();   // the tile's last block has been read
 #pragma unroll
   for (int j = 0; j < 8; ++j)
