@@ -37,6 +37,9 @@ struct DeviceStatus {
   int block;      // blockIdx.x of the reporter
   int detail;
 };
+// A code other than that of a wait that ran out: scales that are no powers of two in an 8-bit tensor not marked so (where: 0 the
+// first operand, 1 the second; detail: k-block).
+constexpr int kStatusScales = 20;
 
 struct Context {
   bool ready = false;

@@ -860,8 +860,20 @@ gemm_q_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
             const float* src = o.s + scale_offset(o, first + h * 128 + i * 32 + lane) + (int64_t)kb0 * o.s_k;
 #pragma unroll
             for (int j = 0; j < kQGroup; ++j)
-              bits[h][i][j] = (h == 0 || for_q) && kb0 + j < num_kb ? __float_as_uint(__ldg(src + j * o.s_k)) : 0u;
+              bits[h][i][j] = (h == 0 || for_q) && kb0 + j < num_kb ? __float_as_uint(__ldg(src + j * o.s_k)) : 0x3f800000u;
           }
+        // The exponent is all that is used of a scale.  One with a sign, a mantissa, or an exponent field of 0 or 255 is no power of
+        // two: the tensor lacks its mark, the product would be wrong, and the host hears of it.
+        uint32_t odd = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < kQGroup; ++j)
+              odd |= (bits[h][i][j] & 0x807fffffu) | ((bits[h][i][j] - 0x00800000u) & 0x80000000u) |
+                     ((bits[h][i][j] + 0x00800000u) & 0x80000000u);
+        if (__any_sync(0xffffffffu, odd != 0) && lane == 0) report(p.t.status, kStatusScales, for_q, kb0);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll

@@ -128,6 +128,10 @@ int check_device_status() {
   DeviceStatus s = *g_ctx.status_host;
   if (s.code == 0) return CLEAVE_CUDA_OK;
   memset(g_ctx.status_host, 0, sizeof(DeviceStatus));
+  if (s.code == kStatusScales)
+    return set_error(CLEAVE_CUDA_ERR_ARG,
+                     "gemm_e4m3: the %s operand has scales that are not positive powers of two (near k-block %d) and is not marked "
+                     "CLEAVE_SCALES_ANY; the product is invalid", s.where ? "second" : "first", s.detail);
   return set_error(CLEAVE_CUDA_ERR_DEVICE_TIMEOUT,
                    "a kernel gave up a bounded wait (code %d, location %d, block %d, detail %d); "
                    "results of the queued work are invalid",

@@ -285,7 +285,8 @@ class QTensor:
     @classmethod
     def from_device_ptr(cls, ptr: int, scales_ptr: int, rows: int, cols: int, blocks: str, any_scales: bool = False) -> "QTensor":
         """Non-owning view of caller-owned device memory: the bytes (16-byte aligned, pitch as above) and the scales.
-        ``any_scales`` has to be set where they are not all positive powers of two: nothing looks at them here."""
+        ``any_scales`` has to be set where they are not all positive powers of two: nothing looks at them here, and a large
+        product of such a tensor fails at the next synchronisation."""
         dims = _q_dims(rows, cols, blocks)
         h = lib().cleave_cuda_wrap_e4m3(ctypes.c_void_p(ptr), lib().cleave_cuda_e4m3_bytes(*dims))
         if not h:

@@ -369,7 +369,8 @@ int32_t cleave_cuda_sgd_f64(cleave_buf w, cleave_buf g, double lr, double gscale
  * Scales are positive powers of two, 2^-126 to 2^127, as cleave_cuda_quantize_e4m3 makes them: large products let the
  * tensor pipe apply them, which reads nothing but a scale's exponent.  A tensor from elsewhere whose scales are other f32
  * values is marked by adding CLEAVE_SCALES_ANY to its block form wherever it is read; its large products take the kernel that
- * multiplies by the scales (about half as fast). */
+ * multiplies by the scales (less than half as fast).  Without the mark a large product fails at the next synchronisation
+ * (CLEAVE_CUDA_ERR_ARG); small ones multiply by the scales anyway. */
 enum { CLEAVE_BLOCKS_ROWS = 1, CLEAVE_BLOCKS_COLS = 2, CLEAVE_BLOCKS_TILES = 3, CLEAVE_SCALES_ANY = 16 };
 int64_t cleave_cuda_e4m3_bytes(int32_t rows, int32_t cols);                     /* length of the byte handle */
 int64_t cleave_cuda_e4m3_scales(int32_t rows, int32_t cols, int32_t blocks);    /* length of the scale handle */
