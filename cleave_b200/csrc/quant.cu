@@ -479,7 +479,7 @@ extern "C" {
 int64_t cleave_cuda_e4m3_bytes(int32_t rows, int32_t cols) { return rows > 0 && cols > 0 ? q_bytes(rows, cols) : 0; }
 
 int64_t cleave_cuda_e4m3_scales(int32_t rows, int32_t cols, int32_t blocks) {
-  return rows > 0 && cols > 0 ? q_scales(rows, cols, blocks) : 0;
+  return rows > 0 && cols > 0 ? q_scales(rows, cols, blocks & ~CLEAVE_SCALES_ANY) : 0;
 }
 
 cleave_buf cleave_cuda_alloc_e4m3(int64_t bytes) {
