@@ -21,12 +21,17 @@ f64 = ctypes.c_double
 i32, i64, f32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 
 
-
 class _Int32:
-    """Converts an ``int32_t`` argument.  ``operator.index`` refuses what is no integer, as ``c_int32`` does, but makes no object of
-    it: an 8-bit product's call, eight of whose fourteen arguments are such, takes 1.3 us instead of 4.4."""
+    """Converts an ``int32_t`` argument to what ``c_int32`` would, but makes no object of an integer: an 8-bit product's call, eight
+    of whose fourteen arguments are such, takes 0.9 us instead of 1.6.  What is no integer goes to ``c_int32``, which takes its own
+    objects and those with an ``_as_parameter_`` and refuses the rest."""
 
-    from_param = operator.index
+    @staticmethod
+    def from_param(value, _index=operator.index):
+        try:
+            return _index(value)
+        except TypeError:
+            return i32.from_param(value)
 
 
 # name -> (restype, argtypes); mirrors include/cleave_cuda.h declaration by declaration.
