@@ -44,8 +44,8 @@ class MLP2:
         again; default: on for layer sizes that are multiples of 32 (what the tensor-core route needs to read
         the tensors in place).  The gradients are bit-identical either way.
         ``products``: ``"f32"``, or ``"e4m3"`` for products of 8-bit operands with a scale per block of 128.  Parameters,
-        activations handed out, loss and gradients stay f32; between the forward and the backward pass the inputs of
-        both layers are kept in 8 bits only, a quarter of the memory, and the backward pass reads them as they are."""
+        activations handed out, loss and gradients stay f32; of the layers' inputs the backward pass reads one 8-bit form
+        each, so that between the passes H takes a quarter of its f32 memory (X's form stands beside the caller's X)."""
         if products not in ("f32", "e4m3"):
             raise ValueError(f"products: 'f32' or 'e4m3', not {products!r}")
         self.products = products
@@ -170,19 +170,24 @@ class MLP2:
         batch = X.dims[0]
         X_rows, X_cols = quantize(X, "rows", "cols")
         H = gemm_q_into(Tensor.empty(batch, self.d_hid), X_rows, quantize(self.W1, "tiles"), bias=self.b1, act=self.act1)
+        X_rows = None   # a form goes with its last reader; its block serves later tensors of the step
         H_rows, H_cols = quantize(H, "rows", "cols")   # H_cols is all that the backward pass keeps of H
         H = H if keep else None
         if before_layer:
             before_layer(2)
         W2 = quantize(self.W2, "tiles")
         Y = gemm_q_into(Tensor.empty(batch, self.d_out), H_rows, W2, bias=self.b2, act=self.act2)
+        H_rows = None
         loss, dZ2 = nn.mse_act_bwd(Y, T, self.act2, loss_out)
         dZ2_rows, dZ2_cols = quantize(dZ2, "rows", "cols")
         dH = gemm_q_into(Tensor.empty(batch, self.d_hid), dZ2_rows, W2, trans_b=True)
+        dZ2_rows = W2 = None
         dZ1_cols = QTensor(batch, self.d_hid, "cols")
         dZ1 = Tensor.empty(batch, self.d_hid) if keep else None
         nn.act_bwd_q(H_cols, dH, self.act1, dZ1_cols, dz=dZ1, db=self.db1)
+        dH = dH if keep else None
         gemm_q_into(self.dW1, X_cols, dZ1_cols, trans_a=True)
+        X_cols = dZ1_cols = None
         if on_grads_ready:
             on_grads_ready(1)
         gemm_q_into(self.dW2, H_cols, dZ2_cols, trans_a=True)
