@@ -170,9 +170,7 @@ class FusedDataParallel:
         # Lo planes of the weights (what the tensor-core products read beside W itself), refreshed on the side stream
         # right after the exchange that rewrote the layer: the split of W1 / W2 leaves the step's critical path.
         # _planes[b] belongs to bucket b's weight matrix; valid only after that bucket's first exchange.
-        self._planes = None
-        if len(self._buckets) == 2:
-            self._planes = [Tensor.empty(*self.net.W2.dims), Tensor.empty(*self.net.W1.dims)]
+        self._planes = _lo_planes(self.net, len(self._buckets))
         self._planes_version = [-1, -1]   # net.weights_version at the refresh; a load() or sgd() since makes a plane stale
 
     def _exchange(self, b: int, lr: float, stream) -> None:
@@ -239,6 +237,14 @@ class FusedDataParallel:
             self._planes_version[b] = self.net.weights_version
         self._done[b].record(self._side)
         self._in_flight[b] = True
+
+
+def _lo_planes(net, buckets: int):
+    """Room for the lo planes of both weight matrices, in bucket order; none where the step's products do not read any."""
+    from .linalg import Tensor
+    if buckets != 2 or getattr(net, "products", "f32") != "f32":
+        return None
+    return [Tensor.empty(*net.W2.dims), Tensor.empty(*net.W1.dims)]
 
 
 class MLP2Replica:
