@@ -499,7 +499,10 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
 #pragma unroll
       for (int e = 0; e < 4; ++e) bias[u][e] = p.bias != nullptr && row[u] < p.m && col[u] + e < p.n ? __ldg(p.bias + col[u] + e) : 0.0f;
     }
-    if (base == 0 && ranks > 1) cluster_sync_all();
+    if (base == 0 && ranks > 1) {
+      __syncwarp();   // the barrier's .aligned form needs the warp in one piece, and the lanes' loads above differ
+      cluster_sync_all();
+    }
     float4 part[kBatch][kQMaxSplit];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u)
@@ -537,8 +540,8 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
       }
     }
   }
+  __syncwarp();
   if (arrived) {
-    __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // the peers have read this CTA's shared memory
   }
   if (warp == 1) {
