@@ -565,10 +565,10 @@ gemm_q_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__
 // in four columns of 32 lanes, repeated in all four lane quarters (tcgen05.cp ... 32x128b.warpx4).  P: the CTA's own 128 rows;
 // Q: all 256, in both CTAs.
 //
-// Measured, 8192^3, 256 MiB of C included: 453 us (2.43 PFLOP/s, 770 clocks a k-block at 1.53 GHz, the power limit; the pipe's own
-// rate is 512), one scale per column or per 128 alike.  A drain that scales every k-block itself (as gemm_q_kernel does), same
-// tile: 577 us with one scale for 128 columns, 1030 us with one per column, the pipe waiting for the drain's multiplies.  What it
-// waits for now: the accumulator's drain at the end of a chunk (about 650 clocks in 4100), and power.
+// Measured, 8192^3, 256 MiB of C included: 440 to 453 us in bursts (2.43 PFLOP/s, 770 clocks a k-block at 1.53 GHz, the power limit; the
+// pipe's own rate is 512) and 520 to 535 us over seconds, one scale per column or per 128 alike.  A drain that scales every k-block
+// itself (as gemm_q_kernel does), same tile: 577 us with one scale for 128 columns, 1030 us with one per column, the pipe waiting for
+// the drain's multiplies.  What it waits for now: the accumulator's drain at the end of a chunk (about 650 clocks in 4100), and power.
 constexpr int kQPairDrainWarps = 16;
 constexpr int kQPairCols = 64;                               // columns a drain warp sums: a quarter of the tile
 constexpr int kQPairThreads = 128 + 32 * kQPairDrainWarps;   // warp 0 TMA, 1 MMA, 2 scales of P, 3 scales of Q
@@ -1077,9 +1077,10 @@ static bool gemm_q_pairs(const QSide& a, const QSide& b, float* c, const float* 
 }
 
 static bool gemm_q(const QSide& a, const QSide& b, float* c, const float* bias, int act) {
-  // CTA pairs from 19 tiles of 256 x 256 on (an eighth of the SMs), unless a side fits half a tile.  Measured, one CTA / pairs, us:
-  // 16 tiles (1024 x 1024) k 512 14.8 / 12.9, k 4096 22.1 / 23.0; 24 tiles (1536 x 1024) 16.9 / 12.9, 31.4 / 23.1; 64 tiles 22.8 /
-  // 13.8, 51.9 / 26.0; 136 x 8192 16.9 / 12.8, 32.1 / 25.1; but 128 x 8192, k 4096 23.2 / 25.1, k 8192 31.4 / 39.2.
+  // CTA pairs from 19 tiles of 256 x 256 on (an eighth of the SMs), unless a side fits half a tile.  Measured, one CTA / pairs, us, B in
+  // tiles: 16 tiles (1024 x 1024) k 512 13.8 / 12.4, k 4096 18.5 / 24.5; 24 tiles (1536 x 1024) 14.4 / 12.4, 26.7 / 24.5; 64 tiles
+  // 18.5 / 14.2, 43.0 / 24.6; 136 x 8192 14.8 / 12.7, 26.7 / 24.6; but 128 x 8192, k 4096 20.4 / 24.6, k 8192 26.7 / 38.0.  A scale
+  // per column of B: 16 tiles k 4096 26.7 / 24.5, 24 tiles 41.0 / 24.6, 128 x 8192, k 8192 41.1 / 39.0.
   const int64_t pair_tiles = (int64_t)ceil_div(a.dim, 256) * ceil_div(b.dim, 256);
   if (!a.any_scales && !b.any_scales && pair_tiles > ctx().sm_count / 8 && pair_tiles <= 0x3fffffff && a.dim > 128 && b.dim > 128)
     return gemm_q_pairs(a, b, c, bias, act);
